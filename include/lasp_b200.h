@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define LASP_B200_ABI_VERSION 4
+#define LASP_B200_ABI_VERSION 5
 
 /* the library is built with hidden visibility; only the entry points below are exported */
 #if defined(__GNUC__)
@@ -330,6 +330,109 @@ LASP_B200_API int lasp_b200_copy_status_async(int32_t* status_host_pinned, void*
  *     forward-only (inference / prefill) entry point. */
 #define LASP_B200_STATIC_SCRATCH_BYTES (64u << 20)
 LASP_B200_API int lasp_b200_forward_static(const lasp_problem* p, const lasp_fwd_args* a, void* stream);
+
+/* ---- recurrences over tokens with a kept state: short causal convolution, selective scan ----------------------------------
+ * (No counterpart in the reference.)  Tensors of tokens are addressed by pitches, in elements, with the channels (or states)
+ * of a token side by side: element (row, token, group, i) lies at data + row * row_pitch + token * token_pitch + group *
+ * group_pitch + i.  Nothing else is asked of their alignment than that of their type; where addresses and pitches are
+ * multiples of 16 bytes loads are wider.
+ *
+ * Sequences: with sequences = 0 every row is one, of `tokens` tokens.  Otherwise rows is 1 and the row is packed: sequence i is
+ * tokens offsets[i] to offsets[i + 1] (device, ascending, index_bits 32 or 64 each; out of range they are clamped), an empty one
+ * among them is allowed, and outputs of tokens that lie in none are written as zeros.
+ *
+ * Steps (one token of every row of a decoding batch) read and write the kept states in place: row r goes by state slots[r]
+ * (index_bits 32 or 64; NULL: r).  A row whose slot is not one of the `slot_count` states leaves every state as it is and gets an
+ * output of zeros.  Rows that name the same slot are consecutive tokens of its sequence, in the order of the rows. */
+typedef struct {
+  void* data;
+  int64_t row_pitch, token_pitch, group_pitch;
+} lasp_tokens;
+
+typedef enum { LASP_ACT_NONE = 0, LASP_ACT_SILU = 1 } lasp_activation;
+
+/* y_t = act(bias + sum_j weight[c][j] x_(t - width + 1 + j)), channel by channel; width 2, 3 or 4.  What lies before a sequence is
+ * its state_in, the last width - 1 inputs, oldest first; state_out those after its last token.  Backward: dx, and whichever of
+ * dweight, dbias, dstate_in are not NULL, from dy and dstate_out (NULL: zero). */
+typedef struct {
+  int32_t rows, tokens, channels, width;
+  int32_t dtype;        /* x, y, dy, dx and the states */
+  int32_t param_dtype;  /* weight, bias and their gradients: LASP_F32 or dtype */
+  int32_t activation;   /* lasp_activation */
+  int32_t sequences, index_bits;
+  const void* offsets;
+  lasp_tokens x, y, dy, dx;
+  const void* weight;    /* (channels, width) */
+  const void* bias;      /* (channels), or NULL */
+  const void* state_in;  /* (sequences, width - 1, channels), or NULL = zeros */
+  void* state_out;       /* or NULL = not wanted */
+  const void* dstate_out;
+  void* dstate_in;
+  void* dweight;
+  void* dbias;
+  void* ws;              /* backward: lasp_b200_conv_workspace_bytes() */
+  size_t ws_bytes;
+} lasp_conv_args;
+LASP_B200_API size_t lasp_b200_conv_workspace_bytes(const lasp_conv_args* a);
+LASP_B200_API int lasp_b200_conv_forward(const lasp_conv_args* a, void* stream);
+LASP_B200_API int lasp_b200_conv_backward(const lasp_conv_args* a, void* stream);
+
+/* h_t = exp(dt_t[c] A[c][n]) h_(t-1) + dt_t[c] u_t[c] B_t[n],  y_t[c] = (sum_n C_t[n] h_t[c][n] + D[c] u_t[c]) silu(z_t[c]), with
+ * dt = softplus(dt + dt_bias) where softplus is set, dt + dt_bias elsewhere; states <= 64.  B and C are shared by the channels /
+ * groups channels of a group.  A, D and the states h (sequences, channels, states) are fp32.  A of an infinity counts as fp32's
+ * largest number.  Backward needs `kept`, which the forward pass leaves (lasp_b200_scan_kept_bytes(); NULL: not wanted). */
+typedef struct {
+  int32_t rows, tokens, channels, states, groups;
+  int32_t dtype;        /* u, dt, z, B, C, y and their gradients */
+  int32_t param_dtype;  /* D, dt_bias and their gradients: LASP_F32 or dtype */
+  int32_t softplus;
+  int32_t sequences, index_bits;
+  const void* offsets;
+  lasp_tokens u, dt, z, B, C, y;      /* z.data NULL = no gate */
+  lasp_tokens dy, du, ddt, dz, dB, dC;
+  const float* A;        /* (channels, states) */
+  const void* D;         /* (channels), or NULL = zeros */
+  const void* dt_bias;   /* (channels), or NULL = zeros */
+  const float* state_in;
+  float* state_out;
+  const float* dstate_out;
+  float* dstate_in;
+  float* dA;             /* each of these may be NULL = not wanted */
+  void* dD;
+  void* ddt_bias;
+  void* kept;
+  size_t kept_bytes;
+  void* ws;              /* backward: lasp_b200_scan_workspace_bytes() */
+  size_t ws_bytes;
+} lasp_scan_args;
+LASP_B200_API size_t lasp_b200_scan_kept_bytes(const lasp_scan_args* a);
+LASP_B200_API size_t lasp_b200_scan_workspace_bytes(const lasp_scan_args* a);
+LASP_B200_API int lasp_b200_scan_forward(const lasp_scan_args* a, void* stream);
+LASP_B200_API int lasp_b200_scan_backward(const lasp_scan_args* a, void* stream);
+
+/* One token of every row; of the tensors of tokens the row and group pitches count. */
+typedef struct {
+  int32_t rows, channels, width, dtype, param_dtype, activation;
+  int32_t slot_count, index_bits;
+  const void* slots;
+  lasp_tokens x, y;
+  const void* weight;
+  const void* bias;
+  void* state;           /* (slot_count, width - 1, channels) */
+} lasp_conv_step_args;
+LASP_B200_API int lasp_b200_conv_step(const lasp_conv_step_args* a, void* stream);
+
+typedef struct {
+  int32_t rows, channels, states, groups, dtype, param_dtype, softplus;
+  int32_t slot_count, index_bits;
+  const void* slots;
+  lasp_tokens u, dt, z, B, C, y;
+  const float* A;
+  const void* D;
+  const void* dt_bias;
+  float* state;          /* (slot_count, channels, states) */
+} lasp_scan_step_args;
+LASP_B200_API int lasp_b200_scan_step(const lasp_scan_step_args* a, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,6 +7,8 @@ from .lasp_fuse import lasp_fuse, lasp_fuse_  # noqa: F401
 from .lasp_fuse_parallel import lasp_fuse_parallel, lasp_fuse_parallel_  # noqa: F401
 from .lasp_naive import lasp_naive, lasp_naive_  # noqa: F401
 from .lightning_attention import lightning_attn, lightning_attn_  # noqa: F401
+from .causal_conv import causal_conv, causal_conv_step  # noqa: F401
+from .selective_scan import selective_scan, selective_scan_step  # noqa: F401
 from .utils import *  # noqa: F401,F403
 from ._core import lightning_attn_fused  # noqa: F401
 from ._core import sequence_parallel_fused as lasp_fuse_parallel_fused  # noqa: F401

@@ -10,7 +10,7 @@ import ctypes as C
 import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "liblasp_b200.so")
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # lasp_dtype / lasp_path / lasp_status of include/lasp_b200.h
 F32, BF16, F16 = 0, 1, 2
@@ -64,6 +64,39 @@ class ExchangeArgs(C.Structure):
                [("peer_slots", C.c_void_p * 8), ("peer_acks", C.c_void_p * 8), ("wait_clocks", C.c_int64)]
 
 
+class Tokens(C.Structure):   # lasp_tokens
+    _fields_ = [("data", C.c_void_p), ("row_pitch", C.c_int64), ("token_pitch", C.c_int64), ("group_pitch", C.c_int64)]
+
+
+def _fields(ints, *rest):
+    """The int32 fields of an argument structure, then its pointers (str), token tensors (tuple of names) and sizes (dict)."""
+    out = [(n, C.c_int32) for n in ints.split()]
+    for r in rest:
+        out += [(n, Tokens) for n in r] if isinstance(r, tuple) else list(r.items()) if isinstance(r, dict) else [(n, C.c_void_p) for n in r.split()]
+    return out
+
+
+class ConvArgs(C.Structure):   # lasp_conv_args
+    _fields_ = _fields("rows tokens channels width dtype param_dtype activation sequences index_bits", "offsets",
+                       ("x", "y", "dy", "dx"), "weight bias state_in state_out dstate_out dstate_in dweight dbias ws", {"ws_bytes": C.c_size_t})
+
+
+class ScanArgs(C.Structure):   # lasp_scan_args
+    _fields_ = _fields("rows tokens channels states groups dtype param_dtype softplus sequences index_bits", "offsets",
+                       ("u", "dt", "z", "B", "C", "y", "dy", "du", "ddt", "dz", "dB", "dC"),
+                       "A D dt_bias state_in state_out dstate_out dstate_in dA dD ddt_bias kept", {"kept_bytes": C.c_size_t}, "ws",
+                       {"ws_bytes": C.c_size_t})
+
+
+class ConvStepArgs(C.Structure):   # lasp_conv_step_args
+    _fields_ = _fields("rows channels width dtype param_dtype activation slot_count index_bits", "slots", ("x", "y"), "weight bias state")
+
+
+class ScanStepArgs(C.Structure):   # lasp_scan_step_args
+    _fields_ = _fields("rows channels states groups dtype param_dtype softplus slot_count index_bits", "slots",
+                       ("u", "dt", "z", "B", "C", "y"), "A D dt_bias state")
+
+
 _PP, _FP, _BP = C.POINTER(Problem), C.POINTER(FwdArgs), C.POINTER(BwdArgs)
 
 # symbol -> (restype, argtypes); every entry point include/lasp_b200.h declares
@@ -100,6 +133,15 @@ SIGNATURES = {
     "lasp_b200_linked_ok": (C.c_int, [_PP]),
     "lasp_b200_forward_linked": (C.c_int, [_PP, _FP, C.POINTER(ExchangeArgs), C.c_void_p]),
     "lasp_b200_bwd_dkv_linked": (C.c_int, [_PP, _BP, C.POINTER(ExchangeArgs), C.c_void_p]),
+    "lasp_b200_conv_workspace_bytes": (C.c_size_t, [C.POINTER(ConvArgs)]),
+    "lasp_b200_conv_forward": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
+    "lasp_b200_conv_backward": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
+    "lasp_b200_conv_step": (C.c_int, [C.POINTER(ConvStepArgs), C.c_void_p]),
+    "lasp_b200_scan_kept_bytes": (C.c_size_t, [C.POINTER(ScanArgs)]),
+    "lasp_b200_scan_workspace_bytes": (C.c_size_t, [C.POINTER(ScanArgs)]),
+    "lasp_b200_scan_forward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
+    "lasp_b200_scan_backward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
+    "lasp_b200_scan_step": (C.c_int, [C.POINTER(ScanStepArgs), C.c_void_p]),
 }
 STATIC_SCRATCH_BYTES = 64 << 20  # LASP_B200_STATIC_SCRATCH_BYTES
 

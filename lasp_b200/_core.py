@@ -142,17 +142,26 @@ def _slices_in_place(q, v, qk_scale, feature_map) -> bool:
 
 _QK_MAPS = {None: 0, "elu1": 1}
 _attention = None   # lasp_b200._torch_ops.attention, looked up at the first call
+_torch_ops = None
+
+
+def native(name):
+    """The native operator of that name (csrc/torch_ops.cpp, csrc/torch_recurrent.cpp)."""
+    global _torch_ops
+    if _torch_ops is None:
+        try:
+            from . import _torch_ops as module
+        except ImportError as exc:
+            from ._cabi import LaspLibraryError
+            raise LaspLibraryError("the native operator lasp_b200/_torch_ops.so is missing or does not load: build it with "
+                                   f"`python -m lasp_b200.build` (there is no fallback): {exc}") from exc
+        _torch_ops = module
+    return getattr(_torch_ops, name)
 
 
 def _load_attention():
     global _attention
-    try:
-        from . import _torch_ops
-    except ImportError as exc:
-        from ._cabi import LaspLibraryError
-        raise LaspLibraryError("the native operator lasp_b200/_torch_ops.so is missing or does not load: build it with "
-                               f"`python -m lasp_b200.build` (there is no fallback): {exc}") from exc
-    _attention = _torch_ops.attention
+    _attention = native("attention")
     return _attention
 
 

@@ -19,7 +19,9 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "liblasp_b200.so")
 TORCH_OPS = os.path.join(PKG, "_torch_ops.so")   # the operator as PyTorch calls it, on top of LIB
-SOURCES = ["api.cu", "split_kernels.cu", "state_kernels.cu", "fault_word.cu", "walk_kernels.cu", "wide_kernels.cu", "relay_kernels.cu", "static_scratch.cu"]
+SOURCES = ["api.cu", "split_kernels.cu", "state_kernels.cu", "fault_word.cu", "walk_kernels.cu", "wide_kernels.cu", "relay_kernels.cu", "static_scratch.cu",
+           "recurrent_api.cu", "conv_kernels.cu", "scan_forward.cu", "scan_backward.cu", "scan_step.cu"]
+TORCH_SOURCES = ["torch_ops.cpp", "torch_recurrent.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -73,21 +75,27 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_torch_ops(force: bool = False) -> None:
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    if not (force or _stale(TORCH_OPS, [src, os.path.join(ROOT, "include", "lasp_b200.h")])):
+    headers = [os.path.join(CSRC, "torch_common.h"), os.path.join(ROOT, "include", "lasp_b200.h")]
+    sources = [os.path.join(CSRC, f) for f in TORCH_SOURCES]
+    if not (force or _stale(TORCH_OPS, sources + headers)):
         return
     import sysconfig
     import torch
     base = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    include = [os.path.join(ROOT, "include"), os.path.join(base, "include"),
+    include = [os.path.join(ROOT, "include"), CSRC, os.path.join(base, "include"),
                os.path.join(base, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"),
                sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wno-interference-size", "-o", TORCH_OPS, src]
-    cmd += [x for d in include for x in ("-I", d)]
-    cmd += ["-L", PKG, "-l:liblasp_b200.so", "-L", os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-            "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
-    subprocess.check_call(cmd)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wno-interference-size"] + [x for d in include for x in ("-I", d)]
+    objs, procs = [src[:-4] + ".torch.o" for src in sources], []
+    for src, obj in zip(sources, objs):
+        if force or _stale(obj, [src] + headers):
+            procs.append(subprocess.Popen(["g++", "-c", src, "-o", obj] + flags))
+    if any([p.wait() for p in procs]):
+        raise RuntimeError("g++ failed")
+    subprocess.check_call(["g++", "-shared", "-o", TORCH_OPS] + objs +
+                          ["-L", PKG, "-l:liblasp_b200.so", "-L", os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch",
+                           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
 
 
 if __name__ == "__main__":

@@ -33,13 +33,19 @@ namespace {
 
 thread_local char g_cuda_error[256] = "";
 
-int cuda_fail(cudaError_t err) {
+}  // namespace
+
+int lasp::status_of(cudaError_t err) {
   if (err == cudaSuccess) return LASP_OK;
   snprintf(g_cuda_error, sizeof(g_cuda_error), "%s%s%s", cudaGetErrorString(err),
            lasp::g_failed_step[0] ? " in " : "", lasp::g_failed_step);
   lasp::g_failed_step = "";
   return LASP_ERR_CUDA;
 }
+
+namespace {
+
+int cuda_fail(cudaError_t err) { return lasp::status_of(err); }
 
 // A thread that has made no CUDA runtime call yet (PyTorch's autograd worker for
 // device 0 is one) has no driver context bound, and the driver-API tensor-map
@@ -184,7 +190,7 @@ const char* lasp_b200_strerror(int status) {
   switch (status) {
     case LASP_OK: return "ok";
     case LASP_ERR_NULL: return "a required pointer is NULL";
-    case LASP_ERR_SHAPE: return "unsupported shape (need b,h,n > 0; d,e multiples of 16 up to 128; b*h <= 65535)";
+    case LASP_ERR_SHAPE: return "unsupported shape (attention: b,h,n > 0; d,e multiples of 16 up to 128; b*h <= 65535)";
     case LASP_ERR_DTYPE: return "unknown dtype";
     case LASP_ERR_ALIGN: return "pointer not 16-byte aligned";
     case LASP_ERR_WORKSPACE: return "workspace too small";

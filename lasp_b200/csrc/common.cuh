@@ -87,6 +87,9 @@ cudaError_t read_fault_word(int32_t* host, bool clear, cudaStream_t st);
 // device address of the current device's fault word (for kernels in other translation units)
 cudaError_t fault_word_address(int32_t** out);
 
+// The status that stands for a CUDA error, whose text lasp_b200_last_cuda_error() then has (api.cu).
+int status_of(cudaError_t err);
+
 // name of the host-side step that produced the last cudaError_t (for error text)
 extern thread_local const char* g_failed_step;
 

@@ -7,21 +7,6 @@
 // (:510-531: a sum over 128-wide q,k slices, v slices side by side): every 128-wide slice pair is read and written
 // where it lies in the wide tensors (row pitch in the problem), later contributions to a slice of o, dq, dk, dv
 // are added by the kernels' own stores.
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/SavedTensorHooks.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/library.h>
-
-#include <nvtx3/nvToolsExt.h>
-
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -31,7 +16,7 @@
 #include <utility>
 #include <vector>
 
-#include "lasp_b200.h"
+#include "torch_common.h"
 
 namespace {
 
@@ -39,53 +24,12 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+using lasp_torch::check_status;
+using lasp_torch::lasp_dtype_of;
+using lasp_torch::Range;
+
 constexpr int64_t kSlice = 128;      // widest q/k (d) or v (e) slice one kernel call takes
 constexpr int64_t kSyncBytes = 4096; // synchronisation words of a launch (lasp_call_options.sync)
-
-struct Range {   // NVTX range around a library call (LASP_B200_NVTX=1)
-  bool on;
-  explicit Range(const char* name) : on(enabled()) {
-    if (on) nvtxRangePushA(name);
-  }
-  ~Range() {
-    if (on) nvtxRangePop();
-  }
-  static bool enabled() {
-    static const bool v = [] {
-      const char* e = std::getenv("LASP_B200_NVTX");
-      return e && e[0] == '1';
-    }();
-    return v;
-  }
-};
-
-// A negative status becomes lasp_b200._cabi.LaspStatusError, on whatever thread this is (autograd's workers too).
-void check_status(const char* fn, int status) {
-  if (status >= 0) return;
-  std::string text = lasp_b200_strerror(status);
-  if (status == LASP_ERR_CUDA) text += std::string(": ") + lasp_b200_last_cuda_error();
-  PyGILState_STATE gil = PyGILState_Ensure();
-  PyObject* mod = PyImport_ImportModule("lasp_b200._cabi");
-  PyObject* cls = mod ? PyObject_GetAttrString(mod, "LaspStatusError") : nullptr;
-  PyObject* exc = cls ? PyObject_CallFunction(cls, "sis", fn, status, text.c_str()) : nullptr;
-  if (exc) PyErr_SetObject(cls, exc);
-  Py_XDECREF(exc);
-  Py_XDECREF(cls);
-  Py_XDECREF(mod);
-  python_error err;
-  err.persist();
-  PyGILState_Release(gil);
-  throw err;
-}
-
-int32_t lasp_dtype_of(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return LASP_F32;
-    case at::kBFloat16: return LASP_BF16;
-    case at::kHalf: return LASP_F16;
-    default: TORCH_CHECK_TYPE(false, "unsupported dtype ", t, "; use float32, bfloat16 or float16");
-  }
-}
 
 int32_t requested_path() {   // env LASP_B200_PATH, looked at on every call as the Python launcher does
   const char* p = std::getenv("LASP_B200_PATH");
@@ -416,6 +360,10 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef kMethods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention)), METH_FASTCALL,
      "attention(q, k, v, s, qk_scale, map) -> o: decay-masked causal linear attention on scale * map(q), scale * map(k)"},
+    {"causal_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lasp_torch::py_causal_conv)), METH_FASTCALL, nullptr},
+    {"causal_conv_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lasp_torch::py_causal_conv_step)), METH_FASTCALL, nullptr},
+    {"selective_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lasp_torch::py_selective_scan)), METH_FASTCALL, nullptr},
+    {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(lasp_torch::py_selective_scan_step)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
