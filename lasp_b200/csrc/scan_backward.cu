@@ -4,43 +4,100 @@
 //   dC_t = sum_c d_t h_t,  dB_t = sum_c g_t dt_t u_t,  du_t = dt_t <g_t, B_t> + D d_t
 //   e_t = a_t g_t h_(t-1):  d dt_t = u_t <g_t, B_t> + <e_t, A>,  dA = sum_t dt_t e_t
 //
-// A block owns a tile of channels of a sequence, as in the forward pass, and walks back along its tokens, kKeep at a time, from the
-// states that the forward pass has kept.  Each warp takes its NT tokens once up to learn three things of them: the product of the
-// decays, the state they leave from zero, and the gradient they pass on from zero (sum_t a_first ... a_t C_t d_t, which runs upwards
-// like the other two).  One exchange between the warps then gives each both what comes from before and what comes from behind;
-// it goes up again for the states and down for the gradients.  dB and dC are sums over channels: each tile leaves its own,
-// and k_scan_sum_tokens adds them up in the order of the tiles, so that results do not depend on when blocks run.
+// Blocks share out their work as in the forward pass (scan_common.cuh) and walk back along the tokens.  The warps that hold the states take a
+// chunk up from the state that the forward pass has kept ahead of it, for the states, and down again for the gradients; its
+// decays stay in registers for both, the states for half a chunk at a time.  dB and dC are sums over channels: each block leaves
+// its tile's, and k_scan_sum_tokens adds those up in the order of the tiles, so that results do not depend on when blocks run.
+#include <type_traits>
+
 #include "scan_common.cuh"
 
 namespace lasp {
 namespace {
 
-template <typename T, int LPC, int CPL, int W, int NT>
+// Sums of 8 numbers of each lane over the warp's channels (lanes that differ in lane % kGroups), for each of the LPC fours of
+// states, to `to[number][four]`.
+//   bf16: products of a matrix of zeros and ones with the numbers rounded to tf32's 11 bits, half of the instructions that exchanges
+//   take.  2^-11 of a term is an eighth of what the sum itself is rounded by; an infinity among a four's numbers makes NaN of the others'
+//   sums too.
+//   fp16, fp32: exchanges.
+template <typename T, int LPC>
+struct ChannelSums {
+  static constexpr int kGroups = 32 / LPC;
+  float one[4][4];   // the matrices' part of this lane: [product][fragment]
+  __device__ __forceinline__ ChannelSums(int lane) {
+    const int row = lane / 4, k = lane % 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {   // fragments: rows below and above 8, columns below and above 4
+        const int r = row + f % 2 * 8, col = k + f / 2 * 4;
+        // two channels: rows 4 q + (0, 1 | 2, 3) pick number 2 q | 2 q + 1 of even and odd fours; else row 2 q | 2 q + 1 picks it
+        const bool picked = LPC == 16 ? r / 4 == q && r % 4 == col / 2 : r / 2 == q && r % 2 == col / 4;
+        one[q][f] = picked ? 1.f : 0.f;
+      }
+  }
+  __device__ __forceinline__ void operator()(float (&v)[8], int lane, float* to) const {
+    if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
+      sum_over<8, kGroups, 1>(v, lane);
+#pragma unroll
+      for (int k = 0; k < 8 / kGroups; ++k) to[(lane % kGroups * (8 / kGroups) + k) * LPC + lane / kGroups] = v[k];
+    } else {
+      float d[4] = {};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t x, y;
+        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(x) : "f"(v[2 * q]));
+        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(v[2 * q + 1]));
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(__float_as_uint(one[q][0])), "r"(__float_as_uint(one[q][1])), "r"(__float_as_uint(one[q][2])), "r"(__float_as_uint(one[q][3])), "r"(x), "r"(y));
+      }
+      const int row = lane / 4, col = lane % 4 * 2;
+      if constexpr (LPC == 4) {
+        to[row * LPC + lane % 4] = d[0] + d[1];   // (both halves of a four's eight channels)
+      } else if constexpr (LPC == 8) {
+        *reinterpret_cast<float2*>(to + row * LPC + col) = make_float2(d[0], d[1]);
+      } else {
+        const int number = row / 4 * 2 + row % 4 / 2, four = 2 * col + row % 2;
+        to[number * LPC + four] = d[0], to[number * LPC + four + 2] = d[1];
+        to[(number + 4) * LPC + four] = d[2], to[(number + 4) * LPC + four + 2] = d[3];
+      }
+    }
+  }
+};
+
+constexpr int kSumsOfToken = 8;   // numbers of a four of states: 4 dB, 4 dC
+template <typename T, int LPC>
 struct Shared {
-  using TILE = Tile<LPC, CPL>;
-  struct Tokens {
-    float dt[NT][TILE::kChannels], dtu[NT][TILE::kChannels], d[NT][TILE::kChannels];
-    float B[NT][TILE::kStates], C[NT][TILE::kStates];
-  } tokens[W];
-  float4 decay[W][CPL][32], state[W][CPL][32], grad[W][CPL][32];
+  using TILE = Tile<LPC>;
+  static constexpr int kStages = sizeof(T) == 4 ? 6 : 8;   // chunks that are here, or on their way, as they are in global memory
+  Vec<T, TILE::kEach> u[kStages][TILE::kUnits], dt[kStages][TILE::kUnits], z[kStages][TILE::kUnits], dy[kStages][TILE::kUnits];
+  Vec<T, 4> B[kStages][TILE::kStateUnits], C[kStages][TILE::kStateUnits];
+  float2 step[3][kChunk][TILE::kChannels];          // dt, dt u
+  float d[3][kChunk][TILE::kChannels];
+  float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
+  float y[2][kChunk][TILE::kChannels + 4], gB[2][kChunk][TILE::kChannels + 4], eA[2][kChunk][TILE::kChannels + 4];   // <C, h>, <g, B>, <e, A>
+  float4 sums[2][kChunk][4][kSumsOfToken * LPC / 4];   // of each warp
+  alignas(16) float skip[TILE::kChannels], bias[TILE::kChannels];
 };
 
 // What a backward pass writes beside its results, in the order of the workspace.
 struct Partial {
-  float* tokens;   // [tile][row * tokens + token][LPC][8]: of 4 states their 4 dB, 4 dC
-  float* rates;    // [sequence][channel][kStates]: dA
-  float* skips;    // [sequence][2][channel]: dD, ddt_bias
+  float4* tokens;   // [tile][row * tokens + token][8][LPC]: of each four of states its 4 dB, 4 dC
+  float4* rates;    // [sequence][tile][kGroup]: dA, as the lanes hold it
+  float* skips;     // [sequence][2][channel]: dD, ddt_bias
 };
 
-template <typename T, int LPC, int CPL, int W, int NT>
-__global__ void __launch_bounds__(32 * W) k_scan_backward(lasp_scan_args a, int tiles, Partial out) {
-  using TILE = Tile<LPC, CPL>;
-  constexpr int kRounds = NT / TILE::kRound, kFill = NT * TILE::kStates / 32, kHalf = 128 * CPL, kShare = 2 * kHalf / (32 * W);
-  constexpr int kLeft = 8 / TILE::kGroups;   // of 8 sums over a warp's channels, how many a lane is left with
-  static_assert(W * NT == kKeep && kShare >= 1 && TILE::kGroups <= 8, "");
-  extern __shared__ char raw_smem[];
-  auto& sm = *reinterpret_cast<Shared<T, LPC, CPL, W, NT>*>(raw_smem);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = lane % LPC, g = lane / LPC;
+// wide: the tensors of tokens can be read and written by kEach, B and C by four.
+template <typename T, int LPC>
+__global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a, int tiles, Partial out, bool wide) {
+  using TILE = Tile<LPC>;
+  using SHARED = Shared<T, LPC>;
+  constexpr int kEach = TILE::kEach, kVecs = TILE::kVecs, kStages = SHARED::kStages, kLead = kStages - 3;
+  extern __shared__ __align__(16) char raw_smem[];
+  auto& sm = *reinterpret_cast<SHARED*>(raw_smem);
+  const int role = threadIdx.x / kGroup, me = threadIdx.x % kGroup;
   const int tile_index = blockIdx.x % tiles, seq = blockIdx.x / tiles;
   const TilePlace<TILE> tile(tile_index, a.channels, a.groups);
   if (a.sequences && seq == a.sequences) {
@@ -48,209 +105,242 @@ __global__ void __launch_bounds__(32 * W) k_scan_backward(lasp_scan_args a, int 
     return;
   }
   const Stretch at = stretch_of(a, seq);
-  const int own = g * CPL + i % CPL, sub = i / CPL;
-  const bool own_ok = own < tile.left;
-  const int64_t own_c = tile.channel + own;
-  const auto rows = [&](const lasp_tokens& t) { return static_cast<T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch; };
-  const T *pu = rows(a.u) + own_c, *pdt = rows(a.dt) + own_c, *pz = a.z.data ? rows(a.z) + own_c : nullptr, *pdy = rows(a.dy) + own_c;
-  const T *pB = rows(a.B) + (int64_t)tile.group * a.B.group_pitch, *pC = rows(a.C) + (int64_t)tile.group * a.C.group_pitch;
-  T *pdu = rows(a.du) + own_c, *pddt = rows(a.ddt) + own_c, *pdz = pz ? rows(a.dz) + own_c : nullptr;
-  float* to_tokens = out.tokens + ((int64_t)tile_index * a.rows * a.tokens + (int64_t)at.row * a.tokens + at.begin) * (2 * TILE::kStates) + i * 8 + g * kLeft;
-  const bool f32 = a.param_dtype == LASP_F32;
-  const float skip = own_ok && a.D ? param<T>(a.D, f32, own_c) : 0.f;
-  const float bias = own_ok && a.dt_bias ? param<T>(a.dt_bias, f32, own_c) : 0.f;
-
-  S4 rate[CPL], drate[CPL];
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) {
-    const int ch = g * CPL + c;
-    rate[c] = ch < tile.left ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
-    drate[c] = splat(0.f);
+  const int chunks = (at.tokens + kChunk - 1) / kChunk;   // number k of them is chunk chunks - 1 - k of the sequence
+  const bool f32 = a.param_dtype == LASP_F32, gated = a.z.data != nullptr, whole = wide && tile.left >= TILE::kChannels;
+  for (int c = threadIdx.x; c < TILE::kChannels; c += kThreads) {
+    const bool there = c < tile.left;
+    sm.skip[c] = there && a.D ? param<T>(a.D, f32, tile.channel + c) : 0.f;
+    sm.bias[c] = there && a.dt_bias ? param<T>(a.dt_bias, f32, tile.channel + c) : 0.f;
   }
-  float dskip = 0.f, dbias = 0.f;
-  // element e of a tile's states: [channel][lane][4]
-  const auto state_at = [&](int e, int* ch, int* n) {
-    const int l = e % 128 / 4;
-    *ch = (l / LPC) * CPL + e / 128, *n = (l % LPC) * 4 + e % 4;
-    return *ch < tile.left && *n < a.states;
+  __syncthreads();
+  const auto rows = [&](const lasp_tokens& t) {
+    return static_cast<T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + tile.channel;
   };
-  // The exchange between the warps, shared out over the threads: items below kHalf are states, upwards from what the forward pass
-  // has kept; those from kHalf on gradients, downwards from what reaches the last state of what is left.
-  float carry[kShare];
+  // Barriers: chunks + 3 of them in every role.
+  if (role == 0) {
+    take_registers<152>();
+    const int lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
+    const bool mine = ch < tile.left;
+    const int64_t state_row = ((int64_t)seq * a.channels + tile.channel + ch) * a.states;
+    const S4 A = mine ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
+    S4 grad = mine && a.dstate_out ? s4(four_of(a.dstate_out + state_row, 4 * i, a.states)) : splat(0.f);   // a_(t+1) g_(t+1)
+    S4 dA = splat(0.f);
+    const float4* kept = static_cast<const float4*>(a.kept) + ((at.chunk + chunks - 1) * tiles + tile_index) * kGroup + me;
+    const ChannelSums<T, LPC> over_channels(lane);
+    constexpr int kHalf = kChunk / 2, kRound = LPC < kHalf ? LPC : kHalf, kSame = LPC / kRound;   // tokens whose sums are made together
+    float4 first = chunks ? *kept : make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();   // the first chunk is here
+    __syncthreads();   // it is prepared
+    __syncthreads();   // the second
+    for (int k = 0, buf = 0; k < chunks; ++k, buf = buf == 2 ? 0 : buf + 1) {
+      const S4 start = s4(first);
+      kept -= (int64_t)tiles * kGroup;
+      if (k + 1 < chunks) first = *kept;
+      S4 decay[kChunk], h[kHalf];
 #pragma unroll
-  for (int k = 0; k < kShare; ++k) {
-    const int e = threadIdx.x + k * 32 * W;
-    int ch, n;
-    carry[k] = e >= kHalf && state_at(e - kHalf, &ch, &n) && a.dstate_out
-                   ? a.dstate_out[((int64_t)seq * a.channels + tile.channel + ch) * a.states + n] : 0.f;
-  }
-
-  auto& my = sm.tokens[warp];
-  for (int chunk = (at.tokens - 1) / kKeep * kKeep; chunk >= 0 && at.tokens > 0; chunk -= kKeep) {
-    const int base = chunk + warp * NT;
-    float u[kRounds], z[kRounds], dy[kRounds], dts[kRounds], slope[kRounds];   // slope: of the step size to what it is made of
+      for (int t = 0; t < kChunk; ++t) {
+        const float dt = sm.step[buf][t][ch].x;
+        decay[t] = exp2(mul(A, f2(dt, dt)));
+      }
+      const auto up = [&](int t, S4 before) {
+        const float in = sm.step[buf][t][ch].y;
+        return fma(decay[t], before, mul(load4(&sm.B4[buf][t][i]), f2(in, in)));
+      };
+      S4 middle = start;
 #pragma unroll
-    for (int k = 0; k < kShare; ++k) {
-      const int e = threadIdx.x + k * 32 * W;
-      int ch, n;
-      if (e < kHalf)
-        carry[k] = state_at(e, &ch, &n) ? static_cast<const float*>(a.kept)[((at.kept + chunk / kKeep) * a.channels + tile.channel + ch) * TILE::kStates + n] : 0.f;
-    }
-    __syncwarp();
+      for (int t = 0; t < kHalf; ++t) middle = up(t, middle);
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int t = r * TILE::kRound + sub;
-      const bool there = base + t < at.tokens && own_ok;
-      const int64_t tt = base + t;
-      u[r] = there ? to_f(pu[tt * a.u.token_pitch]) : 0.f;
-      z[r] = there && pz ? to_f(pz[tt * a.z.token_pitch]) : 0.f;
-      dy[r] = there ? to_f(pdy[tt * a.dy.token_pitch]) : 0.f;
-      const float raw = there ? to_f(pdt[tt * a.dt.token_pitch]) + bias : 0.f;
-      dts[r] = there ? (a.softplus ? softplus(raw) : raw) : 0.f;
-      slope[r] = a.softplus ? sigmoid(raw) : 1.f;
-      my.dt[t][own] = dts[r];
-      my.dtu[t][own] = dts[r] * u[r];
-      my.d[t][own] = pz ? dy[r] * silu(z[r]) : dy[r];
-    }
+      for (int half = 1; half >= 0; --half) {
+        const S4 before = half ? middle : start;
 #pragma unroll
-    for (int k = 0; k < kFill; ++k) {
-      const int t = (lane + 32 * k) / TILE::kStates, n = (lane + 32 * k) % TILE::kStates;
-      const int64_t tt = base + t;
-      const bool there = tt < at.tokens && n < a.states;
-      my.B[t][n] = there ? to_f(pB[tt * a.B.token_pitch + n]) : 0.f;
-      my.C[t][n] = there ? to_f(pC[tt * a.C.token_pitch + n]) : 0.f;
-    }
-    __syncwarp();
-
-    S4 decay[NT][CPL];
-    {
-      S4 p[CPL], s[CPL], q[CPL];
+        for (int t = 0; t < kHalf; ++t) h[t] = up(half * kHalf + t, t ? h[t - 1] : before);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const S4 B = s4(*reinterpret_cast<const float4*>(&my.B[t][4 * i])), C = s4(*reinterpret_cast<const float4*>(&my.C[t][4 * i]));
+        for (int r = kHalf - kRound; r >= 0; r -= kRound) {
+          float y[kRound], gB[kRound], eA[kRound];
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const int ch = g * CPL + c;
-          decay[t][c] = exp2(mul(rate[c], my.dt[t][ch]));
-          const S4 in = mul(B, my.dtu[t][ch]), back = mul(C, my.d[t][ch]);
-          s[c] = t ? fma(decay[t][c], s[c], in) : in;
-          p[c] = t ? mul(p[c], decay[t][c]) : decay[t][c];
-          q[c] = t ? fma(p[c], back, q[c]) : mul(p[c], back);
+          for (int q = kRound - 1; q >= 0; --q) {
+            const int t = half * kHalf + r + q;
+            const float2 step = sm.step[buf][t][ch];
+            const float d = sm.d[buf][t][ch];
+            const S4 B = load4(&sm.B4[buf][t][i]), C = load4(&sm.C4[buf][t][i]), &now = h[r + q];
+            const S4 g = fma(C, f2(d, d), grad), dB = mul(g, f2(step.y, step.y)), dC = mul(now, f2(d, d));
+            y[q] = dot(C, now), gB[q] = dot(B, g);
+            grad = mul(decay[t], g);
+            const S4 e = mul(grad, r + q ? h[r + q - 1] : before);
+            eA[q] = dot(e, A);
+            dA = fma(e, f2(step.x, step.x), dA);
+            float v[8];
+            apart(dB.a, v[0], v[1]), apart(dB.b, v[2], v[3]), apart(dC.a, v[4], v[5]), apart(dC.b, v[6], v[7]);
+            over_channels(v, lane, reinterpret_cast<float*>(sm.sums[k & 1][t][me / 32]));
+          }
+          sum_over<kRound, LPC, TILE::kGroups>(y, lane), sum_over<kRound, LPC, TILE::kGroups>(gB, lane), sum_over<kRound, LPC, TILE::kGroups>(eA, lane);
+          if (kSame == 1 || i % kSame == 0) {
+            const int t = half * kHalf + r + i / kSame;
+            sm.y[k & 1][t][ch] = y[0], sm.gB[k & 1][t][ch] = gB[0], sm.eA[k & 1][t][ch] = eA[0];
+          }
         }
       }
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) sm.decay[warp][c][lane] = f4(p[c]), sm.state[warp][c][lane] = f4(s[c]), sm.grad[warp][c][lane] = f4(q[c]);
+      __syncthreads();
     }
+    if (a.dstate_in && mine) store_four(a.dstate_in + state_row, 4 * i, a.states, f4(grad));
+    out.rates[((int64_t)seq * tiles + tile_index) * kGroup + me] = f4(dA);
+  } else if (role == 1) {
+    give_registers<40>();
+    const int row = me / kVecs, c0 = me % kVecs * kEach;
     __syncthreads();
+    for (int k = 0, buf = 0; k < chunks + 2; ++k, buf = buf == 2 ? 0 : buf + 1) {
+      const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk;
+      if (k < chunks) {
+        if (me < TILE::kUnits) {
+          const bool there = t0 + row < at.tokens;   // behind the end the step is zero: the state stays, and no gradient comes in
+          float dt[kEach], u[kEach], d[kEach];
+          numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.u[stage][me], u), numbers<T, kEach>(sm.dy[stage][me], d);
+          if (gated) {
+            float z[kEach];
+            numbers<T, kEach>(sm.z[stage][me], z);
 #pragma unroll
-    for (int k = 0; k < kShare; ++k) {
-      const int e = threadIdx.x + k * 32 * W;
-      const int at_e = e < kHalf ? e : e - kHalf;
-      float* local = reinterpret_cast<float*>(e < kHalf ? sm.state[0] : sm.grad[W - 1]) + at_e;
-      const float* decay = reinterpret_cast<const float*>(e < kHalf ? sm.decay[0] : sm.decay[W - 1]) + at_e;
-      const int step = e < kHalf ? kHalf : -kHalf;
+            for (int q = 0; q < kEach; ++q) d[q] *= silu(z[q]);
+          }
 #pragma unroll
-      for (int w = 0; w < W; ++w, local += step, decay += step) {
-        const float in = carry[k];
-        carry[k] = fmaf(*decay, in, *local);
-        *local = in;
+          for (int q = 0; q < kEach; q += 2) {
+            F2 s = add2(f2(dt[q], dt[q + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + q])});
+            if (a.softplus) s = softplus(s);
+            float x, y, ix, iy;
+            apart(s, x, y), apart(mul2(s, f2(u[q], u[q + 1])), ix, iy);
+            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + q]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float2*>(&sm.d[buf][row][c0 + q]) = there ? make_float2(d[q], d[q + 1]) : make_float2(0.f, 0.f);
+          }
+        }
+#pragma unroll
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {   // (B's and C's for whole warps each)
+          const int n = v % TILE::kStateUnits;
+          const bool there = t0 + n / LPC < at.tokens;
+          float x[4];
+          numbers<T, 4>(v < TILE::kStateUnits ? sm.B[stage][n] : sm.C[stage][n], x);
+          (v < TILE::kStateUnits ? sm.B4 : sm.C4)[buf][n / LPC][n % LPC] = there ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       }
+      __syncthreads();
     }
+  } else {
+    give_registers<48>();
+    const int row = me / kVecs, c0 = me % kVecs * kEach, left = tile.left - c0;
+    const bool unit = me < TILE::kUnits;
+    const T *pu = rows(a.u) + c0, *pdt = rows(a.dt) + c0, *pz = gated ? rows(a.z) + c0 : nullptr, *pdy = rows(a.dy) + c0;
+    const auto state_rows = [&](const lasp_tokens& t) {
+      return static_cast<const T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + (int64_t)tile.group * t.group_pitch;
+    };
+    const T *pB = state_rows(a.B), *pC = state_rows(a.C);
+    T *pdu = rows(a.du) + c0, *pddt = rows(a.ddt) + c0, *pdz = gated ? rows(a.dz) + c0 : nullptr;
+    constexpr int kSums = kSumsOfToken * LPC / 4;
+    float4* to_tokens = out.tokens + ((int64_t)tile_index * a.rows * a.tokens + (int64_t)at.row * a.tokens + at.begin) * kSums;
+    float dskip[kEach] = {}, dbias[kEach] = {};
+    const auto fetch = [&](int k) {   // (behind the end: the last token, which is not used)
+      if (k < chunks) {
+        const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk;
+        if (unit) {
+          const int64_t t = min(t0 + row, at.tokens - 1);
+          bring<T, kEach>(&sm.u[stage][me], pu + t * a.u.token_pitch, whole, left);
+          bring<T, kEach>(&sm.dt[stage][me], pdt + t * a.dt.token_pitch, whole, left);
+          bring<T, kEach>(&sm.dy[stage][me], pdy + t * a.dy.token_pitch, whole, left);
+          if (gated) bring<T, kEach>(&sm.z[stage][me], pz + t * a.z.token_pitch, whole, left);
+        }
+#pragma unroll
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {
+          const int q = v % TILE::kStateUnits, n = q % LPC * 4;
+          const int64_t t = min(t0 + q / LPC, at.tokens - 1);
+          if (v < TILE::kStateUnits)
+            bring<T, 4>(&sm.B[stage][q], pB + t * a.B.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
+          else
+            bring<T, 4>(&sm.C[stage][q], pC + t * a.C.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
+        }
+      }
+      commit_copies();
+    };
+    const auto finish = [&](int k) {
+      const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk, t = t0 + row;
+#pragma unroll
+      for (int v = me; v < kChunk * kSums; v += kGroup) {   // dB, dC of the tile
+        const int token = v / kSums, q = v % kSums;
+        float4 s = sm.sums[k & 1][token][0][q];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          const float4 x = sm.sums[k & 1][token][w][q];
+          s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+        }
+        if (t0 + token < at.tokens) to_tokens[(int64_t)(t0 + token) * kSums + q] = s;
+      }
+      if (unit && t < at.tokens) {
+        float u[kEach], dt[kEach], d[kEach], x[kEach];
+        numbers<T, kEach>(sm.u[stage][me], u), numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.dy[stage][me], d);
+        if (gated) {
+          float z[kEach];
+          numbers<T, kEach>(sm.z[stage][me], z);
+#pragma unroll
+          for (int q = 0; q < kEach; ++q) {
+            const float s = sigmoid(z[q]), zs = z[q] * s;
+            x[q] = d[q] * fmaf(sm.skip[c0 + q], u[q], sm.y[k & 1][row][c0 + q]) * fmaf(zs, 1.f - s, s);
+            d[q] *= zs;
+          }
+          put_some<T, kEach>(pdz + (int64_t)t * a.dz.token_pitch, x, whole, left);
+        }
+        float gB[kEach], ddt[kEach];
+#pragma unroll
+        for (int q = 0; q < kEach; ++q) {
+          dt[q] += sm.bias[c0 + q];
+          gB[q] = sm.gB[k & 1][row][c0 + q];
+          ddt[q] = fmaf(gB[q], u[q], sm.eA[k & 1][row][c0 + q] * (1.f / kLog2e));
+          if (a.softplus) ddt[q] *= sigmoid(dt[q]);
+          dskip[q] = fmaf(d[q], u[q], dskip[q]), dbias[q] += ddt[q];
+        }
+#pragma unroll
+        for (int q = 0; q < kEach; q += 2) {
+          F2 s = f2(dt[q], dt[q + 1]);
+          if (a.softplus) s = softplus(s);
+          apart(s, dt[q], dt[q + 1]);
+          x[q] = fmaf(gB[q], dt[q], sm.skip[c0 + q] * d[q]), x[q + 1] = fmaf(gB[q + 1], dt[q + 1], sm.skip[c0 + q + 1] * d[q + 1]);
+        }
+        put_some<T, kEach>(pdu + (int64_t)t * a.du.token_pitch, x, whole, left);
+        put_some<T, kEach>(pddt + (int64_t)t * a.ddt.token_pitch, ddt, whole, left);
+      }
+    };
+    // while the states are at number k: finish k - 1, send for k + kLead, wait for k + 3
+#pragma unroll
+    for (int k = 0; k < kLead - 2; ++k) fetch(k);
+    await_copies<kLead - 3>();
     __syncthreads();
-    S4 first[CPL], h[NT][CPL], grad[CPL];   // grad: a_(t+1) g_(t+1)
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) first[c] = s4(sm.state[warp][c][lane]), grad[c] = s4(sm.grad[warp][c][lane]);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const S4 B = s4(*reinterpret_cast<const float4*>(&my.B[t][4 * i]));
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) h[t][c] = fma(decay[t][c], t ? h[t - 1][c] : first[c], mul(B, my.dtu[t][g * CPL + c]));
+    for (int k = -2; k < chunks; ++k) {
+      fetch(k + kLead);
+      if (k > 0) finish(k - 1);
+      await_copies<kLead - 3>();
+      __syncthreads();
     }
+    if (chunks) finish(chunks - 1);
+    // dD and ddt_bias of the tile: the rows of a chunk in their order (the other roles are past their last barrier)
+    float* part = &sm.y[0][0][0];
+    static_assert(sizeof(sm.y) >= 2 * kChunk * TILE::kChannels * sizeof(float), "");
+    asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-    for (int r = kRounds - 1; r >= 0; --r) {
-      float sum_y[LPC], sum_b[LPC], sum_a[LPC];
-#pragma unroll
-      for (int q = TILE::kRound - 1; q >= 0; --q) {
-        const int t = r * TILE::kRound + q;
-        const S4 B = s4(*reinterpret_cast<const float4*>(&my.B[t][4 * i])), C = s4(*reinterpret_cast<const float4*>(&my.C[t][4 * i]));
-        S4 dB = splat(0.f), dC = splat(0.f);
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const int ch = g * CPL + c;
-          const float d = my.d[t][ch];
-          const S4 now = fma(C, d, grad[c]);
-          sum_y[q * CPL + c] = add_up(mul(C, h[t][c]));
-          sum_b[q * CPL + c] = add_up(mul(B, now));
-          dB = fma(now, my.dtu[t][ch], dB);
-          dC = fma(h[t][c], d, dC);
-          grad[c] = mul(decay[t][c], now);
-          const S4 e = mul(grad[c], t ? h[t - 1][c] : first[c]);
-          sum_a[q * CPL + c] = add_up(mul(e, rate[c]));
-          drate[c] = fma(e, my.dt[t][ch], drate[c]);
-        }
-        float v[8] = {dB.a.x, dB.a.y, dB.b.x, dB.b.y, dC.a.x, dC.a.y, dC.b.x, dC.b.y};
-        sum_over<8, TILE::kGroups, LPC>(v, lane);
-        if (base + t < at.tokens) {
-          float* to = to_tokens + (int64_t)(base + t) * (2 * TILE::kStates);
-#pragma unroll
-          for (int k = 0; k < kLeft; ++k) to[k] = v[k];
-        }
-      }
-      sum_over<LPC, LPC, 1>(sum_y, lane);
-      sum_over<LPC, LPC, 1>(sum_b, lane);
-      sum_over<LPC, LPC, 1>(sum_a, lane);
-      const int64_t t = base + r * TILE::kRound + sub;
-      if (t < at.tokens && own_ok) {
-        float d = dy[r];
-        if (pz) {
-          pdz[t * a.dz.token_pitch] = from_f<T>(d * fmaf(skip, u[r], sum_y[0]) * d_silu(z[r]));
-          d *= silu(z[r]);
-        }
-        const float ddt = fmaf(sum_b[0], u[r], sum_a[0] * (1.f / kLog2e)) * slope[r];
-        pdu[t * a.du.token_pitch] = from_f<T>(fmaf(sum_b[0], dts[r], skip * d));
-        pddt[t * a.ddt.token_pitch] = from_f<T>(ddt);
-        dskip = fmaf(d, u[r], dskip), dbias += ddt;
-      }
+    for (int q = 0; q < kEach; ++q)
+      if (unit) part[row * TILE::kChannels + c0 + q] = dskip[q], part[(kChunk + row) * TILE::kChannels + c0 + q] = dbias[q];
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int e = me; e < 2 * TILE::kChannels; e += kGroup) {
+      const int which = e / TILE::kChannels, c = e % TILE::kChannels;
+      float s = 0.f;
+      for (int r = 0; r < kChunk; ++r) s += part[(which * kChunk + r) * TILE::kChannels + c];
+      if (c < tile.left) out.skips[((int64_t)seq * 2 + which) * a.channels + tile.channel + c] = s;
     }
-  }
-#pragma unroll
-  for (int k = 0; k < kShare; ++k) {
-    const int e = threadIdx.x + k * 32 * W;
-    int ch, n;
-    if (a.dstate_in && e >= kHalf && state_at(e - kHalf, &ch, &n)) a.dstate_in[((int64_t)seq * a.channels + tile.channel + ch) * a.states + n] = carry[k];
-  }
-  // what the warps have of dA, dD and ddt_bias, in their order
-  __syncthreads();
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) sm.state[warp][c][lane] = f4(drate[c]);
-  reinterpret_cast<float*>(sm.decay[warp])[lane] = dskip, reinterpret_cast<float*>(sm.decay[warp])[32 + lane] = dbias;
-  __syncthreads();
-  for (int e = threadIdx.x; e < kHalf; e += 32 * W) {
-    int ch, n;
-    const bool there = state_at(e, &ch, &n);
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) s += reinterpret_cast<const float*>(sm.state[w])[e];
-    if (there) out.rates[((int64_t)seq * a.channels + tile.channel + ch) * TILE::kStates + n] = s;
-  }
-  if (threadIdx.x < 2 * TILE::kChannels) {
-    const int which = threadIdx.x / TILE::kChannels, ch = threadIdx.x % TILE::kChannels;
-    float s = 0.f;
-    for (int w = 0; w < W; ++w)
-      for (int q = 0; q < TILE::kRound; ++q)   // the lanes that had this channel
-        s += reinterpret_cast<const float*>(sm.decay[w])[32 * which + (ch / CPL) * LPC + q * CPL + ch % CPL];
-    if (ch < tile.left) out.skips[((int64_t)seq * 2 + which) * a.channels + tile.channel + ch] = s;
   }
 }
 
 // dB, dC of a token: over the tiles of its group, in their order.
 template <typename T>
-__global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const float* part, int tiles, int padded) {
-  const int64_t all = (int64_t)a.rows * a.tokens, wide = 2 * padded, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const float* part, int tiles, int lpc) {
+  const int64_t all = (int64_t)a.rows * a.tokens, wide = 8 * lpc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= all * wide) return;
   const int group = blockIdx.y, in_group = tiles / a.groups;
   const int64_t token = e / wide;
-  const int at = (int)(e % wide), n = at / 8 * 4 + at % 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
+  const int at = (int)(e % wide), number = at / lpc, n = at % lpc * 4 + number % 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
   if (n >= a.states) return;
   float s = 0.f;
   bool inside = true;
@@ -263,67 +353,81 @@ __global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const
 #pragma unroll 8
     for (int k = 0; k < in_group; ++k) s += p[(int64_t)k * all * wide];
   }
-  const lasp_tokens& to = at % 8 < 4 ? a.dB : a.dC;
+  const lasp_tokens& to = number < 4 ? a.dB : a.dC;
   static_cast<T*>(to.data)[(int64_t)row * to.row_pitch + (int64_t)t * to.token_pitch + (int64_t)group * to.group_pitch + n] = from_f<T>(s);
 }
 
-// dA, dD, ddt_bias: over the sequences, in their order.
-template <typename T>
-__global__ void __launch_bounds__(256) k_scan_sum_sequences(lasp_scan_args a, Partial in, int padded, int sequences) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, width = padded + 2;
-  if (e >= a.channels * width) return;
-  const int64_t c = e / width;
-  const int n = (int)(e % width);
-  const bool f32 = a.param_dtype == LASP_F32;
-  float s = 0.f;
-  if (n < padded) {
-    if (n >= a.states || !a.dA) return;
-    for (int q = 0; q < sequences; ++q) s += in.rates[((int64_t)q * a.channels + c) * padded + n];
-    a.dA[c * a.states + n] = s;
-  } else {
-    void* to = n == padded ? a.dD : a.ddt_bias;
-    if (!to) return;
-    for (int q = 0; q < sequences; ++q) s += in.skips[((int64_t)q * 2 + (n - padded)) * a.channels + c];
-    store_param<T>(to, f32, c, s);
+// dA: over the sequences, in their order, a thread for each lane of a tile.
+template <int LPC>
+__global__ void __launch_bounds__(kGroup) k_scan_sum_rates(lasp_scan_args a, const float4* part, int tiles, int sequences) {
+  using TILE = Tile<LPC>;
+  const TilePlace<TILE> tile(blockIdx.x, a.channels, a.groups);
+  const int me = threadIdx.x, lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
+  if (ch >= tile.left) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q = 0; q < sequences; ++q) {
+    const float4 v = part[((int64_t)q * tiles + blockIdx.x) * kGroup + me];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
+  store_four(a.dA + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states, s);
+}
+
+// dD, ddt_bias: the same.
+template <typename T>
+__global__ void __launch_bounds__(256) k_scan_sum_skips(lasp_scan_args a, const float* part, int sequences) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  void* to = blockIdx.y ? a.ddt_bias : a.dD;
+  if (c >= a.channels || !to) return;
+  float s = 0.f;
+  for (int q = 0; q < sequences; ++q) s += part[((int64_t)q * 2 + blockIdx.y) * a.channels + c];
+  store_param<T>(to, a.param_dtype == LASP_F32, c, s);
 }
 
 struct Plan {
-  int tiles, sequences, padded;
+  int tiles, sequences;
   size_t tokens, rates, skips;   // floats
 };
-template <class TILE>
+template <int LPC>
 Plan plan_as(const lasp_scan_args& a) {
   Plan p;
-  p.tiles = tiles_of<TILE>(a.channels, a.groups), p.sequences = a.sequences ? a.sequences : a.rows, p.padded = TILE::kStates;
-  p.tokens = (size_t)p.tiles * a.rows * a.tokens * 2 * p.padded;
-  p.rates = (size_t)p.sequences * a.channels * p.padded, p.skips = (size_t)p.sequences * 2 * a.channels;
+  p.tiles = tiles_of<Tile<LPC>>(a.channels, a.groups), p.sequences = a.sequences ? a.sequences : a.rows;
+  p.tokens = (size_t)p.tiles * a.rows * a.tokens * 8 * LPC;
+  p.rates = (size_t)p.sequences * p.tiles * kGroup * 4, p.skips = (size_t)p.sequences * 2 * a.channels;
   return p;
 }
 
-template <typename T, int LPC, int CPL, int W, int NT>
+template <typename T, int LPC>
 cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
-  constexpr auto kernel = k_scan_backward<T, LPC, CPL, W, NT>;
-  constexpr size_t smem = sizeof(Shared<T, LPC, CPL, W, NT>);
-  const cudaError_t err = opt_in_smem<kernel>(smem);
+  using TILE = Tile<LPC>;
+  constexpr auto kernel = k_scan_backward<T, LPC>;
+  constexpr size_t smem = sizeof(Shared<T, LPC>);
+  const cudaError_t err = ready<kernel>(smem);
   if (err != cudaSuccess) return err;
-  const Plan p = plan_as<Tile<LPC, CPL>>(a);
+  const Plan p = plan_as<LPC>(a);
   float* ws = static_cast<float*>(a.ws);
-  const Partial out{ws, ws + p.tokens, ws + p.tokens + p.rates};
-  kernel<<<(unsigned)(p.tiles * (p.sequences + (a.sequences ? 1 : 0))), 32 * W, smem, st>>>(a, p.tiles, out);
-  const int64_t per_group = (int64_t)a.rows * a.tokens * 2 * p.padded, params = (int64_t)a.channels * (p.padded + 2);
-  if (per_group) k_scan_sum_tokens<T><<<dim3((unsigned)((per_group + 255) / 256), a.groups), 256, 0, st>>>(a, out.tokens, p.tiles, p.padded);
-  if (a.dA || a.dD || a.ddt_bias) k_scan_sum_sequences<T><<<(unsigned)((params + 255) / 256), 256, 0, st>>>(a, out, p.padded, p.sequences);
+  const Partial out{reinterpret_cast<float4*>(ws), reinterpret_cast<float4*>(ws + p.tokens), ws + p.tokens + p.rates};
+  bool wide = (a.channels / a.groups) % TILE::kEach == 0 && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
+  for (const lasp_tokens* t : {&a.u, &a.dt, &a.z, &a.dy, &a.du, &a.ddt, &a.dz}) wide = wide && reads_by<T>(*t, TILE::kEach);
+  kernel<<<(unsigned)(p.tiles * (p.sequences + (a.sequences ? 1 : 0))), kThreads, smem, st>>>(a, p.tiles, out, wide);
+  const int64_t per_group = (int64_t)a.rows * a.tokens * 8 * LPC;
+  if (per_group)
+    k_scan_sum_tokens<T><<<dim3((unsigned)((per_group + 255) / 256), a.groups), 256, 0, st>>>(a, reinterpret_cast<const float*>(out.tokens), p.tiles, LPC);
+  if (a.dA) k_scan_sum_rates<LPC><<<p.tiles, kGroup, 0, st>>>(a, out.rates, p.tiles, p.sequences);
+  if (a.dD || a.ddt_bias) k_scan_sum_skips<T><<<dim3((a.channels + 255) / 256, 2), 256, 0, st>>>(a, out.skips, p.sequences);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t backward_as(const lasp_scan_args& a, cudaStream_t st) {
   switch (padded_states(a.states)) {
-    case 16: return launch<T, 4, 2, 16, 4>(a, st);
-    case 32: return launch<T, 8, 2, 16, 4>(a, st);
-    default: return launch<T, 16, 2, 8, 8>(a, st);
+    case 16: return launch<T, 4>(a, st);
+    case 32: return launch<T, 8>(a, st);
+    default: return launch<T, 16>(a, st);
   }
+}
+Plan plan_of(const lasp_scan_args& a) {
+  const int padded = padded_states(a.states);
+  return padded == 16 ? plan_as<4>(a) : padded == 32 ? plan_as<8>(a) : plan_as<16>(a);
 }
 
 }  // namespace
@@ -331,11 +435,10 @@ cudaError_t backward_as(const lasp_scan_args& a, cudaStream_t st) {
 cudaError_t scan_backward(const lasp_scan_args& a, cudaStream_t st) {
   return a.dtype == LASP_F32 ? backward_as<float>(a, st) : a.dtype == LASP_BF16 ? backward_as<__nv_bfloat16>(a, st) : backward_as<__half>(a, st);
 }
-// The forward pass keeps states of as many numbers as its tiles have.
-size_t scan_kept(const lasp_scan_args& a) { return (size_t)kept_states(a) * a.channels * padded_states(a.states) * sizeof(float); }
+// The forward pass keeps four states of each lane of each tile ahead of each chunk.
+size_t scan_kept(const lasp_scan_args& a) { return (size_t)chunks_of(a) * plan_of(a).tiles * kGroup * sizeof(float4); }
 size_t scan_workspace(const lasp_scan_args& a) {
-  const int padded = padded_states(a.states);
-  const Plan p = padded <= 16 ? plan_as<Tile<4, 2>>(a) : padded == 32 ? plan_as<Tile<8, 2>>(a) : plan_as<Tile<16, 2>>(a);
+  const Plan p = plan_of(a);
   return (p.tokens + p.rates + p.skips) * sizeof(float);
 }
 

@@ -1,93 +1,198 @@
-// The selective scan's tile: how a warp shares the channels and states of a token out among its lanes.
+// What the kernels of the selective scan have in common.
 //
 //   h_t[c][n] = exp(dt_t[c] A[c][n]) h_(t-1)[c][n] + dt_t[c] u_t[c] B_t[n],   y_t[c] = sum_n C_t[n] h_t[c][n] + D[c] u_t[c]
 //
-// A lane holds 4 neighbouring states of each of CPL neighbouring channels: LPC lanes side by side make the states of a group of
-// CPL channels, and the 32 / LPC such groups of a warp kChannels channels in all.  So B and C are read by 4s, and a sum over
-// states or channels is added up within lanes before it crosses them.  Sums over the states of kRound tokens at a time give each
-// lane exactly one (token, channel): the one whose u, dt, z it loads and whose outputs it stores (`sum_over`).
+// A block owns a tile of channels of one sequence and walks along its tokens, kChunk at a time.  Four of its warps hold the states: a
+// lane 4 neighbouring ones of one channel, LPC lanes those of a channel (lanes g, g + 32 / LPC, ...: what belongs to a state is then
+// the same for neighbouring lanes, which shared memory serves at once), a warp 32 / LPC channels.  They do nothing but the recurrence and the sums over it:
+// the exponentials bound it (one for every state of every channel and token, 16 per clock and SM), and a warp that also brought, prepared and
+// finished its tokens spent half its time on the latencies of those.  That is what the other eight warps are for.
 #pragma once
+#include <algorithm>
+
 #include "recurrent.cuh"
 
 namespace lasp {
 
-constexpr int kKeep = 64;   // the forward pass of a training call keeps the state ahead of every 64th token of a sequence
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int LPC, int CPL>
+constexpr int kChunk = 16, kGroup = 128, kThreads = 3 * kGroup;   // warps come in groups of four
+template <int LPC>
 struct Tile {
-  static_assert(CPL <= LPC && 32 % LPC == 0, "a lane's channels are at most the lanes of their states");
   static constexpr int kStates = 4 * LPC;
-  static constexpr int kGroups = 32 / LPC;
-  static constexpr int kChannels = kGroups * CPL;
-  static constexpr int kRound = LPC / CPL;   // tokens x kChannels = 32
+  static constexpr int kGroups = 32 / LPC;            // channels of a warp
+  static constexpr int kChannels = 4 * kGroups;
+  // units in which a chunk's tokens are brought and prepared: kEach channels of a token, 4 numbers of B or of C
+  static constexpr int kEach = kChannels % 8 ? 2 : 4, kVecs = kChannels / kEach, kUnits = kChunk * kVecs;
+  static constexpr int kStateUnits = kChunk * LPC;
 };
+// Registers move from the warps that prepare and finish to those that hold the states.  A block is launched with 3 x 128 x kRegisters
+// (two blocks an SM); the shares add up to no more.
+constexpr int kRegisters = 80;
+template <int N>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Shared memory and, because a warp that takes more registers than there are waits for good, the registers that a kernel is launched with:
+// looked at once for each kernel and device.
+template <auto kernel>
+cudaError_t ready(size_t smem) {
+  static const cudaError_t launched_with = [] {
+    cudaFuncAttributes at;
+    const cudaError_t err = cudaFuncGetAttributes(&at, (const void*)kernel);
+    return err != cudaSuccess ? err : at.numRegs >= kRegisters ? cudaSuccess : cudaErrorInvalidConfiguration;
+  }();
+  return launched_with != cudaSuccess ? launched_with : opt_in_smem<kernel>(smem);
+}
 
+// `BYTES` (4, 8, 16 or 32) from global to shared memory without a register in between.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES > 16) {
+    copy_async<16>(to, from);
+    copy_async<BYTES - 16>(static_cast<char*>(to) + 16, static_cast<const char*>(from) + 16);
+  } else if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(BYTES) : "memory");
+  }
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void await_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+// N neighbouring numbers of a row to shared memory: by one asynchronous copy where that may be (`whole`), else those below `left`.
+template <typename T, int N>
+__device__ __forceinline__ void bring(Vec<T, N>* to, const T* from, bool whole, int left) {
+  if (whole) {
+    copy_async<N * (int)sizeof(T)>(to, from);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) to->v[k] = k < left ? from[k] : from_f<T>(0.f);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void numbers(const Vec<T, N>& from, float (&out)[N]) {
+  const Vec<T, N> v = from;
+#pragma unroll
+  for (int k = 0; k < N; ++k) out[k] = to_f(v.v[k]);
+}
+
+// Arithmetic on pairs, one instruction for two fp32 values.  A pair is kept as the 64 bits that those instructions take: taken apart
+// and put together again it would cost a move each time (a third of all instructions, when it was).
 struct F2 {
-  float x, y;
+  unsigned long long v;
 };
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void apart(F2 p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
 __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   F2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
-      "mov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
   return d;
 }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   F2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return d;
 }
 
-// 4 states of a channel
+// 4 states
 struct S4 {
   F2 a, b;
 };
-__device__ __forceinline__ S4 splat(float x) { return {{x, x}, {x, x}}; }
+__device__ __forceinline__ S4 splat(float x) { return {f2(x, x), f2(x, x)}; }
 __device__ __forceinline__ S4 mul(S4 p, S4 q) { return {mul2(p.a, q.a), mul2(p.b, q.b)}; }
-__device__ __forceinline__ S4 mul(S4 p, float f) { return {mul2(p.a, {f, f}), mul2(p.b, {f, f})}; }
+__device__ __forceinline__ S4 mul(S4 p, F2 f) { return {mul2(p.a, f), mul2(p.b, f)}; }   // (f: the same number twice)
 __device__ __forceinline__ S4 fma(S4 p, S4 q, S4 r) { return {fma2(p.a, q.a, r.a), fma2(p.b, q.b, r.b)}; }
-__device__ __forceinline__ S4 fma(S4 p, float f, S4 r) { return {fma2(p.a, {f, f}, r.a), fma2(p.b, {f, f}, r.b)}; }
-__device__ __forceinline__ S4 s4(float4 v) { return {{v.x, v.y}, {v.z, v.w}}; }
-__device__ __forceinline__ float4 f4(S4 v) { return make_float4(v.a.x, v.a.y, v.b.x, v.b.y); }
+__device__ __forceinline__ S4 fma(S4 p, F2 f, S4 r) { return {fma2(p.a, f, r.a), fma2(p.b, f, r.b)}; }
+__device__ __forceinline__ S4 s4(float4 v) { return {f2(v.x, v.y), f2(v.z, v.w)}; }
+__device__ __forceinline__ float4 f4(S4 s) {
+  float4 v;
+  apart(s.a, v.x, v.y), apart(s.b, v.z, v.w);
+  return v;
+}
+__device__ __forceinline__ S4 load4(const void* p) {   // 16 aligned bytes
+  const ulonglong2 v = *static_cast<const ulonglong2*>(p);
+  return {{v.x}, {v.y}};
+}
+__device__ __forceinline__ void store4(void* p, S4 s) { *static_cast<ulonglong2*>(p) = make_ulonglong2(s.a.v, s.b.v); }
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ S4 exp2(S4 x) { return {{ex2(x.a.x), ex2(x.a.y)}, {ex2(x.b.x), ex2(x.b.y)}}; }
-__device__ __forceinline__ float add_up(S4 v) { return (v.a.x + v.a.y) + (v.b.x + v.b.y); }
+__device__ __forceinline__ F2 exp2(F2 p) {
+  float x, y;
+  apart(p, x, y);
+  return f2(ex2(x), ex2(y));
+}
+__device__ __forceinline__ S4 exp2(S4 x) { return {exp2(x.a), exp2(x.b)}; }
+__device__ __forceinline__ float dot(S4 p, S4 q) {
+  float x, y;
+  apart(fma2(p.b, q.b, mul2(p.a, q.a)), x, y);
+  return x + y;
+}
 
-// v[k] summed over the LANES lanes that differ in the bits from STEP to STEP * LANES / 2; lane (bits / STEP) keeps that of index
-// k = bits / STEP (COUNT = LANES), or COUNT / LANES neighbouring ones in v[0], v[1], ...: half of them change lanes at each step.
+// v[k] summed over the LANES lanes that differ in the bits from STEP to STEP * LANES / 2.  COUNT = LANES: the lane of bits q * STEP is left
+// with the sum of index q in v[0].  More: it is left with COUNT / LANES neighbouring ones; fewer: LANES / COUNT neighbouring lanes have
+// the same one.  Half of the values change lanes at each step, so that LANES - 1 exchanges do for LANES sums.
 template <int COUNT, int LANES, int STEP>
 __device__ __forceinline__ void sum_over(float (&v)[COUNT], int lane) {
   if constexpr (LANES > 1) {
     constexpr int m = LANES / 2 * STEP;
-    const bool upper = lane & m;
-    float half[COUNT / 2];
+    if constexpr (COUNT == 1) {
+      v[0] += __shfl_xor_sync(~0u, v[0], m);
+      sum_over<1, LANES / 2, STEP>(v, lane);
+    } else {
+      const bool upper = lane & m;
+      float half[COUNT / 2];
 #pragma unroll
-    for (int k = 0; k < COUNT / 2; ++k) {
-      const float send = upper ? v[k] : v[k + COUNT / 2], keep = upper ? v[k + COUNT / 2] : v[k];
-      half[k] = keep + __shfl_xor_sync(~0u, send, m);
+      for (int k = 0; k < COUNT / 2; ++k) {
+        const float send = upper ? v[k] : v[k + COUNT / 2], keep = upper ? v[k + COUNT / 2] : v[k];
+        half[k] = keep + __shfl_xor_sync(~0u, send, m);
+      }
+      sum_over<COUNT / 2, LANES / 2, STEP>(half, lane);
+#pragma unroll
+      for (int k = 0; k < COUNT / 2; ++k) v[k] = half[k];
     }
-    sum_over<COUNT / 2, LANES / 2, STEP>(half, lane);
-#pragma unroll
-    for (int k = 0; k < COUNT / 2; ++k) v[k] = half[k];
   }
 }
 
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1].  Small steps need it exact relative to e, not to 1: log(1 + e) =
 // 2 atanh(s) with s = e / (2 + e) <= 1/3, whose series s + s^3/3 + s^5/5 ... is cut where it falls below 2^-26.
+__device__ __forceinline__ F2 softplus(F2 p) {
+  float x, y;
+  apart(p, x, y);
+  const float ex = ex2(-fabsf(x) * kLog2e), ey = ex2(-fabsf(y) * kLog2e);
+  const F2 s = f2(__fdividef(ex, 2.f + ex), __fdividef(ey, 2.f + ey)), q = mul2(s, s);
+  const auto k = [](float c) { return f2(c, c); };
+  F2 t = fma2(q, k(1.f / 13), k(1.f / 11));
+  t = fma2(q, t, k(1.f / 9)), t = fma2(q, t, k(1.f / 7)), t = fma2(q, t, k(1.f / 5)), t = fma2(q, t, k(1.f / 3));
+  t = fma2(mul2(s, q), t, s);
+  return fma2(t, k(2.f), f2(fmaxf(x, 0.f), fmaxf(y, 0.f)));
+}
 __device__ __forceinline__ float softplus(float x) {
-  const float e = expf(-fabsf(x)), s = __fdividef(e, 2.f + e), q = s * s;
-  float p = fmaf(q, 1.f / 13, 1.f / 11);
-  p = fmaf(q, p, 1.f / 9), p = fmaf(q, p, 1.f / 7), p = fmaf(q, p, 1.f / 5), p = fmaf(q, p, 1.f / 3);
-  return fmaxf(x, 0.f) + 2.f * fmaf(s * q, p, s);
+  float r, again;
+  apart(softplus(f2(x, x)), r, again);
+  return r;
 }
 
-// Of a 4 x states row of A, B or a state: 4 from state n on, zeros behind the last one.
+// Of a row of A or of a state: 4 numbers from the n-th on, zeros behind the last one.
 __device__ __forceinline__ float4 four_of(const float* p, int n, int states) {
   if (n + 4 <= states && (reinterpret_cast<uintptr_t>(p + n) & 15) == 0) return *reinterpret_cast<const float4*>(p + n);
   return make_float4(n < states ? p[n] : 0.f, n + 1 < states ? p[n + 1] : 0.f, n + 2 < states ? p[n + 2] : 0.f, n + 3 < states ? p[n + 3] : 0.f);
@@ -107,10 +212,10 @@ __device__ __forceinline__ void store_four(float* p, int n, int states, float4 v
 __device__ __forceinline__ S4 rates(const float* A, int n, int states) {
   const float4 v = four_of(A, n, states);
   const auto one = [](float x) { return isinf(x) ? copysignf(3.402823466e38f, x) : x * kLog2e; };
-  return {{one(v.x), one(v.y)}, {one(v.z), one(v.w)}};
+  return {f2(one(v.x), one(v.y)), f2(one(v.z), one(v.w))};
 }
 
-// Which channels a warp's tile is: tiles do not reach across groups, the last of a group may be cut short.
+// Which channels a block's tile is: tiles do not reach across groups, the last of a group may be cut short.
 template <class TILE>
 struct TilePlace {
   int group, channel, left;   // its group, its first channel, how many channels there are from it to the group's end
@@ -128,22 +233,40 @@ int tiles_of(int channels, int groups) {
   return groups * ((in_group + TILE::kChannels - 1) / TILE::kChannels);
 }
 
-// Where a sequence's tokens lie: row and first token, and the number of its first kept state.  A row of n tokens keeps
-// ceil(n / kKeep) states; packed sequence i those from offsets[i] / kKeep + i on, which leaves room for each.
+// Where a sequence's tokens lie: row and first token, and the number of its first chunk among all chunks, as the kept states are
+// counted.  A row of n tokens has ceil(n / kChunk) of them; packed sequence i those from offsets[i] / kChunk + i on, which leaves
+// room for each.
 struct Stretch {
   int row, begin, tokens;
-  int64_t kept;
+  int64_t chunk;
 };
 __device__ __forceinline__ Stretch stretch_of(const lasp_scan_args& a, int seq) {
-  if (!a.sequences) return {seq, 0, a.tokens, (int64_t)seq * ((a.tokens + kKeep - 1) / kKeep)};
+  if (!a.sequences) return {seq, 0, a.tokens, (int64_t)seq * ((a.tokens + kChunk - 1) / kChunk)};
   int begin, end;
   Sequences{a.offsets, a.index_bits, a.sequences, a.tokens}.bounds(seq, &begin, &end);
-  return {0, begin, end - begin, (int64_t)begin / kKeep + seq};
+  return {0, begin, end - begin, (int64_t)begin / kChunk + seq};
 }
-inline int64_t kept_states(const lasp_scan_args& a) {
-  return a.sequences ? (int64_t)a.tokens / kKeep + a.sequences + 1 : (int64_t)a.rows * ((a.tokens + kKeep - 1) / kKeep);
+inline int64_t chunks_of(const lasp_scan_args& a) {
+  return a.sequences ? (int64_t)a.tokens / kChunk + a.sequences + 1 : (int64_t)a.rows * ((a.tokens + kChunk - 1) / kChunk);
+}
+// n neighbouring numbers (n * sizeof(T) <= 16, or a multiple of 16) of a tensor of tokens can be read and written by one access.
+template <typename T>
+bool reads_by(const lasp_tokens& t, int n) {
+  const int bytes = std::min<int>(16, n * (int)sizeof(T)), items = bytes / (int)sizeof(T);
+  return !t.data || (reinterpret_cast<uintptr_t>(t.data) % bytes == 0 && t.row_pitch % items == 0 && t.token_pitch % items == 0 && t.group_pitch % items == 0);
 }
 inline int padded_states(int states) { return states <= 16 ? 16 : states <= 32 ? 32 : 64; }
+
+template <typename T, int N>
+__device__ __forceinline__ void put_some(T* p, const float (&x)[N], bool whole, int left) {
+  if (whole) {
+    store_vec<T, N>(p, x);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k < left) p[k] = from_f<T>(x[k]);
+  }
+}
 
 // Zeros for the tokens of a packed row that lie in no sequence.
 template <typename T, class TILE>

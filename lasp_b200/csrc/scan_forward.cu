@@ -1,217 +1,206 @@
-// Selective scan over prompts and training batches, forward.  The formulas, and how a warp holds a tile of channels and states, are
-// in scan_common.cuh.
+// Selective scan over prompts and training batches, forward.  How a block shares out its work is in scan_common.cuh.
 //
-// A block owns one tile of channels of one sequence and walks along its tokens, W * NT at a time.  Warp w has the NT tokens from
-// w * NT on: it turns their steps into decays once (the exponentials, which bound the kernel: one for every state of every channel
-// and token, at 16 per clock and SM), and takes them along in registers: first from a state of zero, which with the product of the decays
-// says what these tokens make of any state; then, when the states at the W places are known, for the outputs.
+// One barrier a chunk: while the first four warps take chunk j through the recurrence, the next four prepare chunk j + 2 (step sizes, inputs,
+// B and C as numbers), and the last four finish chunk j - 1 (gate, output), send for chunk j + 5 and wait for chunk j + 3.
 #include "scan_common.cuh"
 
 namespace lasp {
 namespace {
 
-template <typename T, int LPC, int CPL, int W, int NT>
+constexpr int kStages = 8;   // chunks that are here, or on their way, as they are in global memory: j - 1 to j + 5
+template <typename T, int LPC>
 struct Shared {
-  using TILE = Tile<LPC, CPL>;
-  struct Tokens {   // of one warp
-    float dt[NT][TILE::kChannels], dtu[NT][TILE::kChannels];
-    float B[NT][TILE::kStates], C[NT][TILE::kStates];
-  } tokens[W];
-  float4 decay[W > 1 ? W : 1][CPL][32], state[W > 1 ? W : 1][CPL][32];
+  using TILE = Tile<LPC>;
+  Vec<T, TILE::kEach> u[kStages][TILE::kUnits], dt[kStages][TILE::kUnits], z[kStages][TILE::kUnits];
+  Vec<T, 4> B[kStages][TILE::kStateUnits], C[kStages][TILE::kStateUnits];
+  float2 step[3][kChunk][TILE::kChannels];                                          // dt, dt u
+  float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
+  float y[2][kChunk][TILE::kChannels + 4];                                          // <C, h>
+  alignas(16) float skip[TILE::kChannels], bias[TILE::kChannels];
 };
 
-template <typename T, int LPC, int CPL, int W, int NT>
-__global__ void __launch_bounds__(32 * W) k_scan_forward(lasp_scan_args a, int tiles) {
-  using TILE = Tile<LPC, CPL>;
-  constexpr int kRounds = NT / TILE::kRound, kFill = NT * TILE::kStates / 32;
-  static_assert(NT % TILE::kRound == 0 && kKeep % NT == 0, "");
-  extern __shared__ char raw_smem[];
-  auto& sm = *reinterpret_cast<Shared<T, LPC, CPL, W, NT>*>(raw_smem);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, i = lane % LPC, g = lane / LPC;
-  const TilePlace<TILE> tile(blockIdx.x % tiles, a.channels, a.groups);
-  const int seq = blockIdx.x / tiles;
+// wide: u, dt, z, y can be read and written by kEach, B and C by four.
+template <typename T, int LPC>
+__global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, int tiles, bool wide) {
+  using TILE = Tile<LPC>;
+  constexpr int kEach = TILE::kEach, kVecs = TILE::kVecs;
+  extern __shared__ __align__(16) char raw_smem[];
+  auto& sm = *reinterpret_cast<Shared<T, LPC>*>(raw_smem);
+  const int role = threadIdx.x / kGroup, me = threadIdx.x % kGroup;
+  const int tile_index = blockIdx.x % tiles, seq = blockIdx.x / tiles;
+  const TilePlace<TILE> tile(tile_index, a.channels, a.groups);
   if (a.sequences && seq == a.sequences) return fill_outside<T, TILE>(a, a.y, tile);
   const Stretch at = stretch_of(a, seq);
-  // this lane's (token, channel) of a round
-  const int own = g * CPL + i % CPL, sub = i / CPL;
-  const bool own_ok = own < tile.left;
-  const int64_t own_c = tile.channel + own;
-  const auto rows = [&](const lasp_tokens& t) { return static_cast<T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch; };
-  const T *pu = rows(a.u) + own_c, *pdt = rows(a.dt) + own_c, *pz = a.z.data ? rows(a.z) + own_c : nullptr;
-  const T *pB = rows(a.B) + (int64_t)tile.group * a.B.group_pitch, *pC = rows(a.C) + (int64_t)tile.group * a.C.group_pitch;
-  T* py = rows(a.y) + own_c;
-  const bool f32 = a.param_dtype == LASP_F32;
-  const float skip = own_ok && a.D ? param<T>(a.D, f32, own_c) : 0.f;
-  const float bias = own_ok && a.dt_bias ? param<T>(a.dt_bias, f32, own_c) : 0.f;
-
-  S4 rate[CPL];   // of channels g * CPL + c, states 4 i to 4 i + 3
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) {
-    const int ch = g * CPL + c;
-    rate[c] = ch < tile.left ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
+  const int chunks = (at.tokens + kChunk - 1) / kChunk;
+  const bool f32 = a.param_dtype == LASP_F32, gated = a.z.data != nullptr, whole = wide && tile.left >= TILE::kChannels;
+  for (int c = threadIdx.x; c < TILE::kChannels; c += kThreads) {
+    const bool there = c < tile.left;
+    sm.skip[c] = there && a.D ? param<T>(a.D, f32, tile.channel + c) : 0.f;
+    sm.bias[c] = there && a.dt_bias ? param<T>(a.dt_bias, f32, tile.channel + c) : 0.f;
   }
-  // The running state: of one warp in its lanes' own layout (W = 1), else shared out for the scan over the warps.
-  constexpr int kShare = W > 1 ? 128 * CPL / (32 * W) : 1;
-  static_assert(W == 1 || kShare >= 1, "");
-  S4 h[CPL];
-  float carry[kShare];
-  const auto state_at = [&](int e, int64_t* where) {   // element e of a tile's states: [channel][lane][4]
-    const int c = e / 128, l = e % 128 / 4, ch = (l / LPC) * CPL + c, n = (l % LPC) * 4 + e % 4;
-    *where = ((int64_t)seq * a.channels + tile.channel + ch) * a.states + n;
-    return ch < tile.left && n < a.states;
+  __syncthreads();
+  const auto rows = [&](const lasp_tokens& t) {
+    return static_cast<T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + tile.channel;
   };
-  if constexpr (W == 1) {
+  // Barriers: chunks + 3 of them in every role.
+  if (role == 0) {
+    take_registers<144>();
+    const int lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
+    const bool mine = ch < tile.left;
+    const int64_t state_row = ((int64_t)seq * a.channels + tile.channel + ch) * a.states;
+    const S4 A = mine ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
+    S4 h = mine && a.state_in ? s4(four_of(a.state_in + state_row, 4 * i, a.states)) : splat(0.f);
+    float4* kept = a.kept ? static_cast<float4*>(a.kept) + (at.chunk * tiles + tile_index) * kGroup + me : nullptr;
+    constexpr int kTurn = 8, kRound = LPC < kTurn ? LPC : kTurn, kSame = LPC / kRound;   // tokens taken, and summed, at a time
+    S4 decay[kTurn], state[kTurn];   // state: first what a token puts in, then the state behind it
+    const auto ahead = [&](int buf, int t0, int t) {   // of token t0 + t
+      const float2 step = sm.step[buf][t0 + t][ch];
+      decay[t] = exp2(mul(A, f2(step.x, step.x)));
+      state[t] = mul(load4(&sm.B4[buf][t0 + t][i]), f2(step.y, step.y));
+    };
+    __syncthreads();   // chunk 0 is here
+    __syncthreads();   // chunk 0 is prepared
+    __syncthreads();   // chunk 1
+    if (chunks) {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      const int ch = g * CPL + c;
-      h[c] = a.state_in && ch < tile.left ? s4(four_of(a.state_in + ((int64_t)seq * a.channels + tile.channel + ch) * a.states, 4 * i, a.states)) : splat(0.f);
+      for (int t = 0; t < kTurn; ++t) ahead(0, 0, t);
     }
-  } else {
+    int buf = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+      if (kept) *kept = f4(h), kept += (int64_t)tiles * kGroup;
+      const int next = buf == 2 ? 0 : buf + 1;
 #pragma unroll
-    for (int k = 0; k < kShare; ++k) {
-      int64_t where;
-      carry[k] = state_at(threadIdx.x + k * 32 * W, &where) && a.state_in ? a.state_in[where] : 0.f;
-    }
-  }
-
-  T u_next[kRounds], dt_next[kRounds], z_next[kRounds], B_next[kFill], C_next[kFill];
-  const auto fetch = [&](int base) {
+      for (int t0 = 0; t0 < kChunk; t0 += kTurn) {
+        S4 now[kTurn];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int t = base + r * TILE::kRound + sub;
-      if (t < at.tokens && own_ok) {
-        u_next[r] = pu[(int64_t)t * a.u.token_pitch], dt_next[r] = pdt[(int64_t)t * a.dt.token_pitch];
-        if (pz) z_next[r] = pz[(int64_t)t * a.z.token_pitch];
-      }
-    }
+        for (int t = 0; t < kTurn; ++t) h = now[t] = fma(decay[t], h, state[t]);
+        // the next tokens' decays go on beside the sums over these: neither needs the other
 #pragma unroll
-    for (int k = 0; k < kFill; ++k) {
-      const int t = base + (lane + 32 * k) / TILE::kStates, n = (lane + 32 * k) % TILE::kStates;
-      const bool there = t < at.tokens && n < a.states;
-      B_next[k] = there ? pB[(int64_t)t * a.B.token_pitch + n] : from_f<T>(0.f);
-      C_next[k] = there ? pC[(int64_t)t * a.C.token_pitch + n] : from_f<T>(0.f);
-    }
-  };
-  fetch(warp * NT);
-
-  auto& my = sm.tokens[warp];
-  for (int chunk = 0; chunk < at.tokens; chunk += W * NT) {
-    const int base = chunk + warp * NT;
-    float u[kRounds], z[kRounds];
-    __syncwarp();
+        for (int t = 0; t < kTurn; ++t) ahead(t0 + kTurn < kChunk ? buf : next, (t0 + kTurn) % kChunk, t);
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int t = r * TILE::kRound + sub;
-      const bool there = base + t < at.tokens && own_ok;   // behind the end the step is zero: the state stays
-      u[r] = there ? to_f(u_next[r]) : 0.f;
-      z[r] = there && pz ? to_f(z_next[r]) : 0.f;
-      const float raw = there ? to_f(dt_next[r]) + bias : 0.f;
-      const float dt = there ? (a.softplus ? softplus(raw) : raw) : 0.f;
-      my.dt[t][own] = dt;
-      my.dtu[t][own] = dt * u[r];
-    }
+        for (int r = 0; r < kTurn; r += kRound) {
+          float sums[kRound];
 #pragma unroll
-    for (int k = 0; k < kFill; ++k) {
-      const int t = (lane + 32 * k) / TILE::kStates, n = (lane + 32 * k) % TILE::kStates;
-      my.B[t][n] = to_f(B_next[k]), my.C[t][n] = to_f(C_next[k]);
-    }
-    __syncwarp();
-    if (chunk + W * NT < at.tokens) fetch(base + W * NT);
-
-    S4 decay[NT][CPL];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) decay[t][c] = exp2(mul(rate[c], my.dt[t][g * CPL + c]));
-    if constexpr (W > 1) {
-      S4 p[CPL], s[CPL];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const S4 B = s4(*reinterpret_cast<const float4*>(&my.B[t][4 * i]));
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const S4 in = mul(B, my.dtu[t][g * CPL + c]);
-          s[c] = t ? fma(decay[t][c], s[c], in) : in;
-          p[c] = t ? mul(p[c], decay[t][c]) : decay[t][c];
+          for (int t = 0; t < kRound; ++t) sums[t] = dot(load4(&sm.C4[buf][t0 + r + t][i]), now[r + t]);
+          sum_over<kRound, LPC, TILE::kGroups>(sums, lane);
+          if (kSame == 1 || i % kSame == 0) sm.y[chunk & 1][t0 + r + i / kSame][ch] = sums[0];
         }
       }
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) sm.decay[warp][c][lane] = f4(p[c]), sm.state[warp][c][lane] = f4(s[c]);
+      buf = next;
       __syncthreads();
+    }
+    if (a.state_out && mine) store_four(a.state_out + state_row, 4 * i, a.states, f4(h));
+  } else if (role == 1) {
+    give_registers<48>();
+    static_assert(TILE::kUnits <= kGroup, "a thread has at most one unit of each tensor");
+    const int row = me / kVecs, c0 = me % kVecs * kEach;
+    __syncthreads();
+    for (int chunk = 0, buf = 0; chunk < chunks + 2; ++chunk, buf = buf == 2 ? 0 : buf + 1) {
+      const int stage = chunk % kStages, t0 = chunk * kChunk;
+      if (chunk < chunks) {
+        if (me < TILE::kUnits) {
+          const bool there = t0 + row < at.tokens;   // behind the end the step is zero: the state stays
+          float dt[kEach], u[kEach];
+          numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.u[stage][me], u);
 #pragma unroll
-      for (int k = 0; k < kShare; ++k) {
-        const int e = threadIdx.x + k * 32 * W;
+          for (int k = 0; k < kEach; k += 2) {
+            F2 d = add2(f2(dt[k], dt[k + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + k])});
+            if (a.softplus) d = softplus(d);
+            float x, y, ix, iy;
+            apart(d, x, y), apart(mul2(d, f2(u[k], u[k + 1])), ix, iy);
+            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + k]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          float* local = reinterpret_cast<float*>(sm.state[w]) + e;
-          const float in = carry[k];
-          carry[k] = fmaf(reinterpret_cast<const float*>(sm.decay[w])[e], in, *local);
-          *local = in;
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {   // (B's and C's for whole warps each)
+          const int k = v % TILE::kStateUnits;
+          const bool there = t0 + k / LPC < at.tokens;
+          float x[4];
+          numbers<T, 4>(v < TILE::kStateUnits ? sm.B[stage][k] : sm.C[stage][k], x);
+          (v < TILE::kStateUnits ? sm.B4 : sm.C4)[buf][k / LPC][k % LPC] = there ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
       __syncthreads();
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) h[c] = s4(sm.state[warp][c][lane]);
     }
-    if (a.kept && base % kKeep == 0 && base < at.tokens) {
-      float4* to = static_cast<float4*>(a.kept) + ((at.kept + base / kKeep) * a.channels + tile.channel) * LPC;
+  } else {
+    give_registers<48>();
+    const int row = me / kVecs, c0 = me % kVecs * kEach, left = tile.left - c0;
+    const bool unit = me < TILE::kUnits;
+    const T *pu = rows(a.u) + c0, *pdt = rows(a.dt) + c0, *pz = gated ? rows(a.z) + c0 : nullptr;
+    const auto state_rows = [&](const lasp_tokens& t) {
+      return static_cast<const T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + (int64_t)tile.group * t.group_pitch;
+    };
+    const T *pB = state_rows(a.B), *pC = state_rows(a.C);
+    T* py = rows(a.y) + c0;
+    const auto fetch = [&](int chunk) {   // (behind the end: the last token, which is not used)
+      const int stage = chunk % kStages, t0 = chunk * kChunk;
+      if (chunk < chunks) {
+        if (unit) {
+          const int64_t t = min(t0 + row, at.tokens - 1);
+          bring<T, kEach>(&sm.u[stage][me], pu + t * a.u.token_pitch, whole, left);
+          bring<T, kEach>(&sm.dt[stage][me], pdt + t * a.dt.token_pitch, whole, left);
+          if (gated) bring<T, kEach>(&sm.z[stage][me], pz + t * a.z.token_pitch, whole, left);
+        }
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (g * CPL + c < tile.left) to[(int64_t)(g * CPL + c) * LPC + i] = f4(h[c]);
-    }
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      float sums[LPC];
-#pragma unroll
-      for (int q = 0; q < TILE::kRound; ++q) {
-        const int t = r * TILE::kRound + q;
-        const S4 B = s4(*reinterpret_cast<const float4*>(&my.B[t][4 * i])), C = s4(*reinterpret_cast<const float4*>(&my.C[t][4 * i]));
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          h[c] = fma(decay[t][c], h[c], mul(B, my.dtu[t][g * CPL + c]));
-          sums[q * CPL + c] = add_up(mul(C, h[c]));
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {
+          const int k = v % TILE::kStateUnits, n = k % LPC * 4;
+          const int64_t t = min(t0 + k / LPC, at.tokens - 1);
+          if (v < TILE::kStateUnits)
+            bring<T, 4>(&sm.B[stage][k], pB + t * a.B.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
+          else
+            bring<T, 4>(&sm.C[stage][k], pC + t * a.C.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
         }
       }
-      sum_over<LPC, LPC, 1>(sums, lane);
-      const int t = base + r * TILE::kRound + sub;
-      if (t < at.tokens && own_ok) {
-        const float y = fmaf(skip, u[r], sums[0]);
-        py[(int64_t)t * a.y.token_pitch] = from_f<T>(pz ? y * silu(z[r]) : y);
+      commit_copies();
+    };
+    const auto finish = [&](int chunk) {
+      const int stage = chunk % kStages, t = chunk * kChunk + row;
+      if (!unit) return;
+      float y[kEach], u[kEach], z[kEach];
+      numbers<T, kEach>(sm.u[stage][me], u);
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) y[k] = fmaf(sm.skip[c0 + k], u[k], sm.y[chunk & 1][row][c0 + k]);
+      if (gated) {
+        numbers<T, kEach>(sm.z[stage][me], z);
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) y[k] *= silu(z[k]);
       }
+      if (t < at.tokens) put_some<T, kEach>(py + (int64_t)t * a.y.token_pitch, y, whole, left);
+    };
+    fetch(0), fetch(1), fetch(2);
+    await_copies<2>();
+    __syncthreads();
+    for (int chunk = -2; chunk < chunks; ++chunk) {
+      fetch(chunk + 5);
+      if (chunk > 0) finish(chunk - 1);
+      await_copies<2>();   // chunk + 3 is here
+      __syncthreads();
     }
-  }
-  if (!a.state_out) return;
-  if constexpr (W == 1) {
-#pragma unroll
-    for (int c = 0; c < CPL; ++c)
-      if (g * CPL + c < tile.left) store_four(a.state_out + ((int64_t)seq * a.channels + tile.channel + g * CPL + c) * a.states, 4 * i, a.states, f4(h[c]));
-  } else {
-#pragma unroll
-    for (int k = 0; k < kShare; ++k) {
-      int64_t where;
-      if (state_at(threadIdx.x + k * 32 * W, &where)) a.state_out[where] = carry[k];
-    }
+    if (chunks) finish(chunks - 1);
   }
 }
 
-template <typename T, int LPC, int CPL, int W, int NT>
+template <typename T, int LPC>
 cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
-  constexpr auto kernel = k_scan_forward<T, LPC, CPL, W, NT>;
-  constexpr size_t smem = sizeof(Shared<T, LPC, CPL, W, NT>);
-  const cudaError_t err = opt_in_smem<kernel>(smem);
+  using TILE = Tile<LPC>;
+  constexpr auto kernel = k_scan_forward<T, LPC>;
+  constexpr size_t smem = sizeof(Shared<T, LPC>);
+  const cudaError_t err = ready<kernel>(smem);
   if (err != cudaSuccess) return err;
-  const int tiles = tiles_of<Tile<LPC, CPL>>(a.channels, a.groups);
+  const int tiles = tiles_of<TILE>(a.channels, a.groups);
   const int sequences = a.sequences ? a.sequences + 1 : a.rows;   // (one more: what lies in none)
-  kernel<<<(unsigned)(tiles * sequences), 32 * W, smem, st>>>(a, tiles);
+  const bool wide = (a.channels / a.groups) % TILE::kEach == 0 && reads_by<T>(a.u, TILE::kEach) && reads_by<T>(a.dt, TILE::kEach) &&
+                    reads_by<T>(a.z, TILE::kEach) && reads_by<T>(a.y, TILE::kEach) && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
+  kernel<<<(unsigned)(tiles * sequences), kThreads, smem, st>>>(a, tiles, wide);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t forward_as(const lasp_scan_args& a, cudaStream_t st) {
   switch (padded_states(a.states)) {
-    case 16: return launch<T, 4, 2, 1, 8>(a, st);
-    case 32: return launch<T, 8, 2, 1, 8>(a, st);
-    default: return launch<T, 16, 2, 1, 8>(a, st);
+    case 16: return launch<T, 4>(a, st);
+    case 32: return launch<T, 8>(a, st);
+    default: return launch<T, 16>(a, st);
   }
 }
 

@@ -55,8 +55,9 @@ __global__ void __launch_bounds__(128) k_scan_step(lasp_scan_step_args a) {
         B = make_float4(at(pB, 0), at(pB, 1), at(pB, 2), at(pB, 3));
         C = make_float4(at(pC, 0), at(pC, 1), at(pC, 2), at(pC, 3));
       }
-      h[k] = fma(exp2(mul(rate[k], dt)), h[k], mul(s4(B), dt * u));
-      float y = add_up(mul(h[k], s4(C)));
+      const float in = dt * u;
+      h[k] = fma(exp2(mul(rate[k], f2(dt, dt))), h[k], mul(s4(B), f2(in, in)));
+      float y = dot(h[k], s4(C));
 #pragma unroll
       for (int m = 1; m < LPC; m *= 2) y += __shfl_xor_sync(~0u, y, m);
       if (there && i == 0) {
