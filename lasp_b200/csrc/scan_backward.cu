@@ -5,77 +5,24 @@
 //   e_t = a_t g_t h_(t-1):  d dt_t = u_t <g_t, B_t> + <e_t, A>,  dA = sum_t dt_t e_t
 //
 // Blocks share out their work as in the forward pass (scan_common.cuh) and walk back along the tokens.  The warps that hold the states take a
-// chunk up from the state that the forward pass has kept ahead of it, for the states, and down again for the gradients; its
-// decays stay in registers for both, the states for half a chunk at a time.  dB and dC are sums over channels: each block leaves
+// chunk up from the state that the forward pass has kept ahead of it, and then half a chunk at a time: up for the states, down for the
+// gradients, with the decays and states of eight tokens in registers.  (Those of 16 do not fit, and a state kept for every eighth
+// token would cost 32 bytes of memory for every eight tokens and state more than the 8 exponentials that the first half takes twice.)  dB and dC are sums over channels: each block leaves
 // its tile's, and k_scan_sum_tokens adds those up in the order of the tiles, so that results do not depend on when blocks run.
-#include <type_traits>
-
 #include "scan_common.cuh"
 
 namespace lasp {
 namespace {
 
-// Sums of 8 numbers of each lane over the warp's channels (lanes that differ in lane % kGroups), for each of the LPC fours of
-// states, to `to[number][four]`.
-//   bf16: products of a matrix of zeros and ones with the numbers rounded to tf32's 11 bits, half of the instructions that exchanges
-//   take.  2^-11 of a term is an eighth of what the sum itself is rounded by; an infinity among a four's numbers makes NaN of the others'
-//   sums too.
-//   fp16, fp32: exchanges.
-template <typename T, int LPC>
-struct ChannelSums {
-  static constexpr int kGroups = 32 / LPC;
-  float one[4][4];   // the matrices' part of this lane: [product][fragment]
-  __device__ __forceinline__ ChannelSums(int lane) {
-    const int row = lane / 4, k = lane % 4;
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int f = 0; f < 4; ++f) {   // fragments: rows below and above 8, columns below and above 4
-        const int r = row + f % 2 * 8, col = k + f / 2 * 4;
-        // two channels: rows 4 q + (0, 1 | 2, 3) pick number 2 q | 2 q + 1 of even and odd fours; else row 2 q | 2 q + 1 picks it
-        const bool picked = LPC == 16 ? r / 4 == q && r % 4 == col / 2 : r / 2 == q && r % 2 == col / 4;
-        one[q][f] = picked ? 1.f : 0.f;
-      }
-  }
-  __device__ __forceinline__ void operator()(float (&v)[8], int lane, float* to) const {
-    if constexpr (!std::is_same<T, __nv_bfloat16>::value) {
-      sum_over<8, kGroups, 1>(v, lane);
-#pragma unroll
-      for (int k = 0; k < 8 / kGroups; ++k) to[(lane % kGroups * (8 / kGroups) + k) * LPC + lane / kGroups] = v[k];
-    } else {
-      float d[4] = {};
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t x, y;
-        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(x) : "f"(v[2 * q]));
-        asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(v[2 * q + 1]));
-        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(__float_as_uint(one[q][0])), "r"(__float_as_uint(one[q][1])), "r"(__float_as_uint(one[q][2])), "r"(__float_as_uint(one[q][3])), "r"(x), "r"(y));
-      }
-      const int row = lane / 4, col = lane % 4 * 2;
-      if constexpr (LPC == 4) {
-        to[row * LPC + lane % 4] = d[0] + d[1];   // (both halves of a four's eight channels)
-      } else if constexpr (LPC == 8) {
-        *reinterpret_cast<float2*>(to + row * LPC + col) = make_float2(d[0], d[1]);
-      } else {
-        const int number = row / 4 * 2 + row % 4 / 2, four = 2 * col + row % 2;
-        to[number * LPC + four] = d[0], to[number * LPC + four + 2] = d[1];
-        to[(number + 4) * LPC + four] = d[2], to[(number + 4) * LPC + four + 2] = d[3];
-      }
-    }
-  }
-};
-
 constexpr int kSumsOfToken = 8;   // numbers of a four of states: 4 dB, 4 dC
 template <typename T, int LPC>
 struct Shared {
   using TILE = Tile<LPC>;
-  static constexpr int kStages = sizeof(T) == 4 ? 6 : 8;   // chunks that are here, or on their way, as they are in global memory
+  static constexpr int kStages = sizeof(T) == 4 ? 6 : 7;   // chunks that are here, or on their way, as they are in global memory
   Vec<T, TILE::kEach> u[kStages][TILE::kUnits], dt[kStages][TILE::kUnits], z[kStages][TILE::kUnits], dy[kStages][TILE::kUnits];
   Vec<T, 4> B[kStages][TILE::kStateUnits], C[kStages][TILE::kStateUnits];
-  float2 step[3][kChunk][TILE::kChannels];          // dt, dt u
-  float d[3][kChunk][TILE::kChannels];
+  float4 step[3][kChunk][TILE::kChannels];          // dt, dt, dt u, dt u: in pairs, as packed operations take them
+  float2 d[3][kChunk][TILE::kChannels];             // d, d
   float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
   float y[2][kChunk][TILE::kChannels + 4], gB[2][kChunk][TILE::kChannels + 4], eA[2][kChunk][TILE::kChannels + 4];   // <C, h>, <g, B>, <e, A>
   float4 sums[2][kChunk][4][kSumsOfToken * LPC / 4];   // of each warp
@@ -84,7 +31,7 @@ struct Shared {
 
 // What a backward pass writes beside its results, in the order of the workspace.
 struct Partial {
-  float4* tokens;   // [tile][row * tokens + token][8][LPC]: of each four of states its 4 dB, 4 dC
+  float4* tokens;   // [tile][row * tokens + token][LPC][8]: of each four of states its 4 dB, 4 dC
   float4* rates;    // [sequence][tile][kGroup]: dA, as the lanes hold it
   float* skips;     // [sequence][2][channel]: dD, ddt_bias
 };
@@ -126,8 +73,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
     S4 grad = mine && a.dstate_out ? s4(four_of(a.dstate_out + state_row, 4 * i, a.states)) : splat(0.f);   // a_(t+1) g_(t+1)
     S4 dA = splat(0.f);
     const float4* kept = static_cast<const float4*>(a.kept) + ((at.chunk + chunks - 1) * tiles + tile_index) * kGroup + me;
-    const ChannelSums<T, LPC> over_channels(lane);
-    constexpr int kHalf = kChunk / 2, kRound = LPC < kHalf ? LPC : kHalf, kSame = LPC / kRound;   // tokens whose sums are made together
+    constexpr int kLeft = 8 / TILE::kGroups;   // of 8 sums over a warp's channels, how many a lane is left with
+    constexpr int kHalf = kChunk / 2, kRound = 4, kSame = LPC / kRound;   // tokens whose sums are made together
     float4 first = chunks ? *kept : make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();   // the first chunk is here
     __syncthreads();   // it is prepared
@@ -136,44 +83,47 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
       const S4 start = s4(first);
       kept -= (int64_t)tiles * kGroup;
       if (k + 1 < chunks) first = *kept;
-      S4 decay[kChunk], h[kHalf];
+      S4 decay[kHalf], h[kHalf];
+      const auto decays = [&](int t0) {
 #pragma unroll
-      for (int t = 0; t < kChunk; ++t) {
-        const float dt = sm.step[buf][t][ch].x;
-        decay[t] = exp2(mul(A, f2(dt, dt)));
-      }
-      const auto up = [&](int t, S4 before) {
-        const float in = sm.step[buf][t][ch].y;
-        return fma(decay[t], before, mul(load4(&sm.B4[buf][t][i]), f2(in, in)));
+        for (int t = 0; t < kHalf; ++t) decay[t] = exp2(mul(A, pair_of(&sm.step[buf][t0 + t][ch])));
+      };
+      const auto up = [&](int t0, int t, S4 before) {
+        return fma(decay[t], before, mul(load4(&sm.B4[buf][t0 + t][i]), pair_of(reinterpret_cast<const float2*>(&sm.step[buf][t0 + t][ch]) + 1)));
       };
       S4 middle = start;
+      decays(0);
 #pragma unroll
-      for (int t = 0; t < kHalf; ++t) middle = up(t, middle);
+      for (int t = 0; t < kHalf; ++t) middle = up(0, t, middle);
 #pragma unroll
       for (int half = 1; half >= 0; --half) {
         const S4 before = half ? middle : start;
+        decays(half * kHalf);
 #pragma unroll
-        for (int t = 0; t < kHalf; ++t) h[t] = up(half * kHalf + t, t ? h[t - 1] : before);
+        for (int t = 0; t < kHalf; ++t) h[t] = up(half * kHalf, t, t ? h[t - 1] : before);
 #pragma unroll
         for (int r = kHalf - kRound; r >= 0; r -= kRound) {
-          float y[kRound], gB[kRound], eA[kRound];
+          float y[kRound], gB[kRound], eA[kRound], over[kRound][kLeft];   // (all stored together: what lies in between could not be read ahead)
 #pragma unroll
           for (int q = kRound - 1; q >= 0; --q) {
             const int t = half * kHalf + r + q;
-            const float2 step = sm.step[buf][t][ch];
-            const float d = sm.d[buf][t][ch];
-            const S4 B = load4(&sm.B4[buf][t][i]), C = load4(&sm.C4[buf][t][i]), &now = h[r + q];
-            const S4 g = fma(C, f2(d, d), grad), dB = mul(g, f2(step.y, step.y)), dC = mul(now, f2(d, d));
+            const S4 step = load4(&sm.step[buf][t][ch]), B = load4(&sm.B4[buf][t][i]), C = load4(&sm.C4[buf][t][i]), &now = h[r + q];
+            const F2 d = pair_of(&sm.d[buf][t][ch]);
+            const S4 g = fma(C, d, grad), dB = mul(g, step.b), dC = mul(now, d);
             y[q] = dot(C, now), gB[q] = dot(B, g);
-            grad = mul(decay[t], g);
+            grad = mul(decay[r + q], g);
             const S4 e = mul(grad, r + q ? h[r + q - 1] : before);
             eA[q] = dot(e, A);
-            dA = fma(e, f2(step.x, step.x), dA);
+            dA = fma(e, step.a, dA);
             float v[8];
             apart(dB.a, v[0], v[1]), apart(dB.b, v[2], v[3]), apart(dC.a, v[4], v[5]), apart(dC.b, v[6], v[7]);
-            over_channels(v, lane, reinterpret_cast<float*>(sm.sums[k & 1][t][me / 32]));
+            sum_over<8, TILE::kGroups, 1>(v, lane);
+#pragma unroll
+            for (int x = 0; x < kLeft; ++x) over[q][x] = v[x];
           }
           sum_over<kRound, LPC, TILE::kGroups>(y, lane), sum_over<kRound, LPC, TILE::kGroups>(gB, lane), sum_over<kRound, LPC, TILE::kGroups>(eA, lane);
+#pragma unroll
+          for (int q = 0; q < kRound; ++q) store_vec<float, kLeft>(reinterpret_cast<float*>(sm.sums[k & 1][half * kHalf + r + q][me / 32]) + lane * kLeft, over[q]);
           if (kSame == 1 || i % kSame == 0) {
             const int t = half * kHalf + r + i / kSame;
             sm.y[k & 1][t][ch] = y[0], sm.gB[k & 1][t][ch] = gB[0], sm.eA[k & 1][t][ch] = eA[0];
@@ -185,13 +135,60 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
     if (a.dstate_in && mine) store_four(a.dstate_in + state_row, 4 * i, a.states, f4(grad));
     out.rates[((int64_t)seq * tiles + tile_index) * kGroup + me] = f4(dA);
   } else if (role == 1) {
+    // while the states are at number k: prepare k + 2, send for k + kLead, add up k - 1
     give_registers<40>();
-    const int row = me / kVecs, c0 = me % kVecs * kEach;
-    __syncthreads();
-    for (int k = 0, buf = 0; k < chunks + 2; ++k, buf = buf == 2 ? 0 : buf + 1) {
-      const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk;
+    const int row = me / kVecs, c0 = me % kVecs * kEach, left = tile.left - c0;
+    const bool unit = me < TILE::kUnits;
+    constexpr int kSums = kSumsOfToken * LPC / 4;
+    float4* to_tokens = out.tokens + ((int64_t)tile_index * a.rows * a.tokens + (int64_t)at.row * a.tokens + at.begin) * kSums;
+    const auto state_rows = [&](const lasp_tokens& t) {
+      return static_cast<const T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + (int64_t)tile.group * t.group_pitch;
+    };
+    const auto fetch = [&](int k) {   // (behind the end: the last token, which is not used)
       if (k < chunks) {
-        if (me < TILE::kUnits) {
+        const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk;
+        if (unit) {
+          const int64_t t = min(t0 + row, at.tokens - 1);
+          bring<T, kEach>(&sm.u[stage][me], rows(a.u) + t * a.u.token_pitch + c0, whole, left);
+          bring<T, kEach>(&sm.dt[stage][me], rows(a.dt) + t * a.dt.token_pitch + c0, whole, left);
+          bring<T, kEach>(&sm.dy[stage][me], rows(a.dy) + t * a.dy.token_pitch + c0, whole, left);
+          if (gated) bring<T, kEach>(&sm.z[stage][me], rows(a.z) + t * a.z.token_pitch + c0, whole, left);
+        }
+#pragma unroll
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {   // (B's and C's for whole warps each)
+          const int q = v % TILE::kStateUnits, n = q % LPC * 4;
+          const int64_t t = min(t0 + q / LPC, at.tokens - 1);
+          if (v < TILE::kStateUnits)
+            bring<T, 4>(&sm.B[stage][q], state_rows(a.B) + t * a.B.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
+          else
+            bring<T, 4>(&sm.C[stage][q], state_rows(a.C) + t * a.C.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
+        }
+      }
+      commit_copies();
+    };
+    const auto add_up = [&](int k) {   // dB, dC of the tile
+      const int t0 = (chunks - 1 - k) * kChunk;
+#pragma unroll
+      for (int v = me; v < kChunk * kSums; v += kGroup) {
+        const int token = v / kSums, q = v % kSums;
+        float4 s = sm.sums[k & 1][token][0][q];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          const float4 x = sm.sums[k & 1][token][w][q];
+          s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+        }
+        if (t0 + token < at.tokens) to_tokens[(int64_t)(t0 + token) * kSums + q] = s;
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kLead - 2; ++k) fetch(k);
+    __syncthreads();
+    for (int k = -2, buf = 0; k < chunks; ++k, buf = buf == 2 ? 0 : buf + 1) {
+      fetch(k + kLead);
+      await_copies<kLead - 2>();   // k + 2 is here, as far as this thread has brought it
+      const int stage = (k + 2) % kStages, t0 = (chunks - 3 - k) * kChunk;
+      if (k + 2 < chunks) {
+        if (unit) {
           const bool there = t0 + row < at.tokens;   // behind the end the step is zero: the state stays, and no gradient comes in
           float dt[kEach], u[kEach], d[kEach];
           numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.u[stage][me], u), numbers<T, kEach>(sm.dy[stage][me], d);
@@ -207,12 +204,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
             if (a.softplus) s = softplus(s);
             float x, y, ix, iy;
             apart(s, x, y), apart(mul2(s, f2(u[q], u[q + 1])), ix, iy);
-            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + q]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float2*>(&sm.d[buf][row][c0 + q]) = there ? make_float2(d[q], d[q + 1]) : make_float2(0.f, 0.f);
+            sm.step[buf][row][c0 + q] = there ? make_float4(x, x, ix, ix) : make_float4(0.f, 0.f, 0.f, 0.f);
+            sm.step[buf][row][c0 + q + 1] = there ? make_float4(y, y, iy, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(&sm.d[buf][row][c0 + q]) = there ? make_float4(d[q], d[q], d[q + 1], d[q + 1]) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
 #pragma unroll
-        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {   // (B's and C's for whole warps each)
+        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {
           const int n = v % TILE::kStateUnits;
           const bool there = t0 + n / LPC < at.tokens;
           float x[4];
@@ -220,99 +218,57 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
           (v < TILE::kStateUnits ? sm.B4 : sm.C4)[buf][n / LPC][n % LPC] = there ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
+      if (k > 0) add_up(k - 1);
       __syncthreads();
     }
+    if (chunks) add_up(chunks - 1);
   } else {
     give_registers<48>();
     const int row = me / kVecs, c0 = me % kVecs * kEach, left = tile.left - c0;
     const bool unit = me < TILE::kUnits;
-    const T *pu = rows(a.u) + c0, *pdt = rows(a.dt) + c0, *pz = gated ? rows(a.z) + c0 : nullptr, *pdy = rows(a.dy) + c0;
-    const auto state_rows = [&](const lasp_tokens& t) {
-      return static_cast<const T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + (int64_t)tile.group * t.group_pitch;
-    };
-    const T *pB = state_rows(a.B), *pC = state_rows(a.C);
-    T *pdu = rows(a.du) + c0, *pddt = rows(a.ddt) + c0, *pdz = gated ? rows(a.dz) + c0 : nullptr;
-    constexpr int kSums = kSumsOfToken * LPC / 4;
-    float4* to_tokens = out.tokens + ((int64_t)tile_index * a.rows * a.tokens + (int64_t)at.row * a.tokens + at.begin) * kSums;
     float dskip[kEach] = {}, dbias[kEach] = {};
-    const auto fetch = [&](int k) {   // (behind the end: the last token, which is not used)
-      if (k < chunks) {
-        const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk;
-        if (unit) {
-          const int64_t t = min(t0 + row, at.tokens - 1);
-          bring<T, kEach>(&sm.u[stage][me], pu + t * a.u.token_pitch, whole, left);
-          bring<T, kEach>(&sm.dt[stage][me], pdt + t * a.dt.token_pitch, whole, left);
-          bring<T, kEach>(&sm.dy[stage][me], pdy + t * a.dy.token_pitch, whole, left);
-          if (gated) bring<T, kEach>(&sm.z[stage][me], pz + t * a.z.token_pitch, whole, left);
-        }
-#pragma unroll
-        for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {
-          const int q = v % TILE::kStateUnits, n = q % LPC * 4;
-          const int64_t t = min(t0 + q / LPC, at.tokens - 1);
-          if (v < TILE::kStateUnits)
-            bring<T, 4>(&sm.B[stage][q], pB + t * a.B.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
-          else
-            bring<T, 4>(&sm.C[stage][q], pC + t * a.C.token_pitch + n, wide && n + 4 <= a.states, a.states - n);
-        }
-      }
-      commit_copies();
-    };
     const auto finish = [&](int k) {
-      const int stage = k % kStages, t0 = (chunks - 1 - k) * kChunk, t = t0 + row;
-#pragma unroll
-      for (int v = me; v < kChunk * kSums; v += kGroup) {   // dB, dC of the tile
-        const int token = v / kSums, q = v % kSums;
-        float4 s = sm.sums[k & 1][token][0][q];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) {
-          const float4 x = sm.sums[k & 1][token][w][q];
-          s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
-        }
-        if (t0 + token < at.tokens) to_tokens[(int64_t)(t0 + token) * kSums + q] = s;
-      }
-      if (unit && t < at.tokens) {
-        float u[kEach], dt[kEach], d[kEach], x[kEach];
-        numbers<T, kEach>(sm.u[stage][me], u), numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.dy[stage][me], d);
-        if (gated) {
-          float z[kEach];
-          numbers<T, kEach>(sm.z[stage][me], z);
-#pragma unroll
-          for (int q = 0; q < kEach; ++q) {
-            const float s = sigmoid(z[q]), zs = z[q] * s;
-            x[q] = d[q] * fmaf(sm.skip[c0 + q], u[q], sm.y[k & 1][row][c0 + q]) * fmaf(zs, 1.f - s, s);
-            d[q] *= zs;
-          }
-          put_some<T, kEach>(pdz + (int64_t)t * a.dz.token_pitch, x, whole, left);
-        }
-        float gB[kEach], ddt[kEach];
+      const int stage = k % kStages, t = (chunks - 1 - k) * kChunk + row;
+      if (!unit || t >= at.tokens) return;
+      float u[kEach], dt[kEach], d[kEach], x[kEach];
+      numbers<T, kEach>(sm.u[stage][me], u), numbers<T, kEach>(sm.dy[stage][me], d);
+      if (gated) {
+        float z[kEach];
+        numbers<T, kEach>(sm.z[stage][me], z);
 #pragma unroll
         for (int q = 0; q < kEach; ++q) {
-          dt[q] += sm.bias[c0 + q];
-          gB[q] = sm.gB[k & 1][row][c0 + q];
-          ddt[q] = fmaf(gB[q], u[q], sm.eA[k & 1][row][c0 + q] * (1.f / kLog2e));
-          if (a.softplus) ddt[q] *= sigmoid(dt[q]);
-          dskip[q] = fmaf(d[q], u[q], dskip[q]), dbias[q] += ddt[q];
+          const float s = sigmoid(z[q]), zs = z[q] * s;
+          x[q] = d[q] * fmaf(sm.skip[c0 + q], u[q], sm.y[k & 1][row][c0 + q]) * fmaf(zs, 1.f - s, s);
+          d[q] *= zs;
         }
-#pragma unroll
-        for (int q = 0; q < kEach; q += 2) {
-          F2 s = f2(dt[q], dt[q + 1]);
-          if (a.softplus) s = softplus(s);
-          apart(s, dt[q], dt[q + 1]);
-          x[q] = fmaf(gB[q], dt[q], sm.skip[c0 + q] * d[q]), x[q + 1] = fmaf(gB[q + 1], dt[q + 1], sm.skip[c0 + q + 1] * d[q + 1]);
-        }
-        put_some<T, kEach>(pdu + (int64_t)t * a.du.token_pitch, x, whole, left);
-        put_some<T, kEach>(pddt + (int64_t)t * a.ddt.token_pitch, ddt, whole, left);
+        put_some<T, kEach>(rows(a.dz) + (int64_t)t * a.dz.token_pitch + c0, x, whole, left);
       }
-    };
-    // while the states are at number k: finish k - 1, send for k + kLead, wait for k + 3
+      numbers<T, kEach>(sm.dt[stage][me], dt);
 #pragma unroll
-    for (int k = 0; k < kLead - 2; ++k) fetch(k);
-    await_copies<kLead - 3>();
+      for (int q = 0; q < kEach; q += 2) {
+        F2 s = add2(f2(dt[q], dt[q + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + q])});
+        float raw[2], step[2];
+        apart(s, raw[0], raw[1]);
+        if (a.softplus) s = softplus(s);
+        apart(s, step[0], step[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float gB = sm.gB[k & 1][row][c0 + q + e];
+          float ddt = fmaf(gB, u[q + e], sm.eA[k & 1][row][c0 + q + e] * (1.f / kLog2e));
+          if (a.softplus) ddt *= sigmoid(raw[e]);
+          dskip[q + e] = fmaf(d[q + e], u[q + e], dskip[q + e]), dbias[q + e] += ddt;
+          x[q + e] = fmaf(gB, step[e], sm.skip[c0 + q + e] * d[q + e]);
+          dt[q + e] = ddt;
+        }
+      }
+      put_some<T, kEach>(rows(a.du) + (int64_t)t * a.du.token_pitch + c0, x, whole, left);
+      put_some<T, kEach>(rows(a.ddt) + (int64_t)t * a.ddt.token_pitch + c0, dt, whole, left);
+    };
     __syncthreads();
-    for (int k = -2; k < chunks; ++k) {
-      fetch(k + kLead);
-      if (k > 0) finish(k - 1);
-      await_copies<kLead - 3>();
+    __syncthreads();
+    __syncthreads();
+    for (int k = 0; k < chunks; ++k) {
+      if (k) finish(k - 1);
       __syncthreads();
     }
     if (chunks) finish(chunks - 1);
@@ -340,7 +296,7 @@ __global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const
   if (e >= all * wide) return;
   const int group = blockIdx.y, in_group = tiles / a.groups;
   const int64_t token = e / wide;
-  const int at = (int)(e % wide), number = at / lpc, n = at % lpc * 4 + number % 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
+  const int at = (int)(e % wide), number = at % 8, n = at / 8 * 4 + number % 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
   if (n >= a.states) return;
   float s = 0.f;
   bool inside = true;

@@ -130,6 +130,7 @@ __device__ __forceinline__ S4 load4(const void* p) {   // 16 aligned bytes
   const ulonglong2 v = *static_cast<const ulonglong2*>(p);
   return {{v.x}, {v.y}};
 }
+__device__ __forceinline__ F2 pair_of(const void* p) { return {*static_cast<const unsigned long long*>(p)}; }   // 8 aligned bytes
 __device__ __forceinline__ void store4(void* p, S4 s) { *static_cast<ulonglong2*>(p) = make_ulonglong2(s.a.v, s.b.v); }
 __device__ __forceinline__ float ex2(float x) {
   float r;

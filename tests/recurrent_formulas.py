@@ -110,11 +110,10 @@ def scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, state=Non
     return out
 
 
-def within(got, want, size, steps, terms=0.0):
+def within(got, want, size, steps):
     """Whether got is the rounded want: half a step of its type relative to the value (for fp16, half of its smallest step at
     least), and for the fp32 arithmetic before, `steps` roundings of 2^-22 (two units, as the fast exponential and division have)
-    relative to the sizes of what is added up.  terms: what each term itself is rounded by before it is added in fp32; the
-    errors of the terms add up to at most that much of the sum of their sizes.  Returns the worst excess, at most 1."""
+    relative to the sizes of what is added up.  Returns the worst excess, at most 1."""
     finfo = torch.finfo(got.dtype)
-    room = finfo.eps / 2 * want.abs() + (steps * 2.0 ** -22 + terms) * size + finfo.smallest_normal * finfo.eps
+    room = finfo.eps / 2 * want.abs() + steps * 2.0 ** -22 * size + finfo.smallest_normal * finfo.eps
     return float(((got.double() - want).abs() / room).max()) if got.numel() else 0.0

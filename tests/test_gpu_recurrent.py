@@ -21,9 +21,7 @@ def _close(got, want, size, steps, names=None):
     for name in names or got:
         if got[name] is not None:
             assert got[name].shape == want[name].shape, (name, got[name].shape, want[name].shape)
-            # dB and dC of bf16 tensors add up products that are rounded to 11 bits (as fp16 has: 2^-11 of each; scan_backward.cu)
-            terms = torch.finfo(F16).eps / 2 if name in ("dB", "dC") and got[name].dtype == BF16 else 0.0
-            off = F.within(got[name], want[name], size[name], steps, terms)
+            off = F.within(got[name], want[name], size[name], steps)
             assert off <= 1.0, (name, off)
 
 
