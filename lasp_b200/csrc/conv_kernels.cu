@@ -3,9 +3,11 @@
 //   p_t = bias + sum_j w_j x_(t-W+1+j),  y_t = p_t or silu(p_t)
 //   dp_t = dy_t silu'(p_t),  dx_t = sum_k w_(W-1-k) dp_(t+k),  dw_j = sum_t dp_t x_(t-W+1+j)
 //
-// A thread owns V neighbouring channels (16 bytes) and a run of tokens: the last W - 1 inputs slide through its registers, so
-// that every input is read once but for the W - 1 ahead of a run.  What bounds it is memory; nothing is staged.
+// A thread owns V neighbouring channels and a run of tokens: the last W - 1 inputs slide through its registers, so that every input is
+// read once but for the W - 1 ahead of a run.  Nothing is staged.  Memory and the issue of instructions bound it: forward
+// 8 x 2048 x 4096 bf16 66 us (41 us at the copy rate), backward 131 us (62).
 #include <algorithm>
+#include <type_traits>
 
 #include "recurrent.cuh"
 
@@ -13,41 +15,59 @@ namespace lasp {
 namespace {
 
 constexpr int kVecs = 32, kRuns = 8;   // a block: 32 vectors of channels times 8 runs of tokens
-constexpr int kBatch = 8;              // tokens whose loads are under way together
-
-struct Rows {   // where a thread's channels of a row of tokens lie
-  int64_t row, token;
-};
+constexpr int kBatch = 8, kBatchBack = 4;   // tokens whose loads are under way together
 
 template <typename T, int V, int W>
 struct Taps {
-  float w[W][V];
-  __device__ __forceinline__ void load(const lasp_conv_args& a, int c) {
+  Channels<V> w[W], bias;
+  template <class ARGS>
+  __device__ __forceinline__ void load(const ARGS& a, int c) {
     const bool f32 = a.param_dtype == LASP_F32;
+    float x[W + 1][2 * Channels<V>::kPairs] = {};
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      if (f32 && W == 4 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0) {
+        const float4 w4 = reinterpret_cast<const float4*>(a.weight)[c + i];
+        x[0][i] = w4.x, x[1][i] = w4.y, x[2 % W][i] = w4.z, x[3 % W][i] = w4.w;
+      } else {
 #pragma unroll
-      for (int j = 0; j < W; ++j) w[j][i] = param<T>(a.weight, f32, (int64_t)(c + i) * W + j);
+        for (int j = 0; j < W; ++j) x[j][i] = param<T>(a.weight, f32, (int64_t)(c + i) * W + j);
+      }
+      if (a.bias) x[W][i] = param<T>(a.bias, f32, c + i);
+    }
+#pragma unroll
+    for (int k = 0; k < Channels<V>::kPairs; ++k) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j].p[k] = f2(x[j][2 * k], x[j][2 * k + 1]);
+      bias.p[k] = f2(x[W][2 * k], x[W][2 * k + 1]);
+    }
+  }
+  // of pair k: bias + the sum over the taps
+  __device__ __forceinline__ F2 sum(const Channels<V> (&past)[W - 1], F2 now, int k) const {
+    F2 p = fma2(w[W - 1].p[k], now, bias.p[k]);
+#pragma unroll
+    for (int m = 0; m < W - 1; ++m) p = fma2(w[m].p[k], past[m].p[k], p);
+    return p;
   }
 };
-
-template <typename T, int V>
-__device__ __forceinline__ void load_bias(const void* bias, int param_dtype, int c, float (&out)[V]) {
+template <int V, int W>
+__device__ __forceinline__ void move_on(Channels<V> (&past)[W], const Channels<V>& now) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = bias ? param<T>(bias, param_dtype == LASP_F32, c + i) : 0.f;
+  for (int m = 0; m + 1 < W; ++m) past[m] = past[m + 1];
+  past[W - 1] = now;
 }
 
 // x at token p of a sequence that begins at `begin`; what lies before is its state, or zero
 template <typename T, int V, int W>
-__device__ __forceinline__ void input_at(const T* x, int64_t pitch, const T* state, int64_t c_total, int begin, int p, float (&out)[V]) {
-  if (p >= begin) {
-    load_vec<T, V>(x + (int64_t)p * pitch, out);
-  } else if (state && p - begin + W - 1 >= 0) {
-    load_vec<T, V>(state + (int64_t)(p - begin + W - 1) * c_total, out);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = 0.f;
-  }
+__device__ __forceinline__ Channels<V> input_at(const T* x, int64_t pitch, const T* state, int64_t c_total, int begin, int p) {
+  Channels<V> out;
+  if (p >= begin)
+    out.load(x + (int64_t)p * pitch);
+  else if (state && p - begin + W - 1 >= 0)
+    out.load(state + (int64_t)(p - begin + W - 1) * c_total);
+  else
+    out.clear();
+  return out;
 }
 
 // The sequence that a thread is in.  `state` is the address of its channels in the state of that sequence.
@@ -86,15 +106,13 @@ __device__ void write_state(const lasp_conv_args& a, int row, int seq, int c) {
   const T* from = a.state_in ? static_cast<const T*>(a.state_in) + (int64_t)seq * (W - 1) * a.channels + c : nullptr;
   T* to = static_cast<T*>(a.state_out) + (int64_t)seq * (W - 1) * a.channels + c;
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m) {
-    float v[V];
-    input_at<T, V, W>(x, a.x.token_pitch, from, a.channels, begin, end - (W - 1) + m, v);
-    store_vec<T, V>(to + (int64_t)m * a.channels, v);
-  }
+  for (int m = 0; m < W - 1; ++m)
+    input_at<T, V, W>(x, a.x.token_pitch, from, a.channels, begin, end - (W - 1) + m).store(to + (int64_t)m * a.channels);
 }
 
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kVecs* kRuns) k_conv_forward(lasp_conv_args a, int run, int blocks_of_runs) {
+__global__ void __launch_bounds__(kVecs* kRuns, 5) k_conv_forward(lasp_conv_args a, int run, int blocks_of_runs) {
+  constexpr int kPairs = Channels<V>::kPairs;
   const int c = (blockIdx.x * kVecs + threadIdx.x) * V, row = blockIdx.z;
   if (c >= a.channels) return;
   if ((int)blockIdx.y >= blocks_of_runs) {   // the states after the last tokens
@@ -109,48 +127,53 @@ __global__ void __launch_bounds__(kVecs* kRuns) k_conv_forward(lasp_conv_args a,
   T* y = static_cast<T*>(a.y.data) + (int64_t)row * a.y.row_pitch + c;
   Taps<T, V, W> taps;
   taps.load(a, c);
-  float bias[V];
-  load_bias<T, V>(a.bias, a.param_dtype, c, bias);
   Place<T, W> at;
   at.start(a, row, t0);
-  float past[W - 1][V];   // past[m]: x_(t-W+1+m)
+  Channels<V> past[W - 1];   // past[m]: x_(t-W+1+m)
+  const auto look_back = [&](int t) {
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m)
-    input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, t0 - (W - 1) + m, past[m]);
-  for (int t = t0; t < t1; t += kBatch) {
+    for (int m = 0; m < W - 1; ++m)
+      past[m] = input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, t - (W - 1) + m);
+  };
+  look_back(t0);
+  // kBatch tokens from t on; `whole`: all of them in this run and, where sequences are packed, in one sequence
+  const auto batch = [&](int t, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
     Vec<T, V> in[kBatch];
+    const T* from = x + (int64_t)t * a.x.token_pitch;
+    T* to = y + (int64_t)t * a.y.token_pitch;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (t + j < t1) in[j] = *reinterpret_cast<const Vec<T, V>*>(x + (int64_t)(t + j) * a.x.token_pitch);
+    for (int j = 0; j < kBatch; ++j, from += a.x.token_pitch)
+      if (kWhole || t + j < t1) in[j] = *reinterpret_cast<const Vec<T, V>*>(from);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (t + j >= t1) break;
+      if (!kWhole && t + j >= t1) break;
       bool inside = true;
-      if (a.sequences) {
+      if (!kWhole && a.sequences) {
         if (t + j >= at.end) {
           at.advance(t + j);
-          if (t + j >= at.begin) {
-#pragma unroll
-            for (int m = 0; m < W - 1; ++m)
-              input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, t + j - (W - 1) + m, past[m]);
-          }
+          if (t + j >= at.begin) look_back(t + j);
         }
         inside = at.inside(t + j);
       }
-      float now[V], out[V];
+      Channels<V> now, out;
+      now.set(in[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        now[i] = to_f(in[j].v[i]);
-        float p = fmaf(taps.w[W - 1][i], now[i], bias[i]);
-#pragma unroll
-        for (int m = 0; m < W - 1; ++m) p = fmaf(taps.w[m][i], past[m][i], p);
-        out[i] = inside ? (a.activation == LASP_ACT_SILU ? silu(p) : p) : 0.f;
-#pragma unroll
-        for (int m = 0; m + 1 < W - 1; ++m) past[m][i] = past[m + 1][i];
-        past[W - 2][i] = now[i];
+      for (int k = 0; k < kPairs; ++k) {
+        const F2 p = taps.sum(past, now.p[k], k);
+        out.p[k] = a.activation == LASP_ACT_SILU ? silu(p) : p;
       }
-      store_vec<T, V>(y + (int64_t)(t + j) * a.y.token_pitch, out);
+      if (!inside) out.clear();
+      move_on(past, now);
+      out.store(to);
+      to += a.y.token_pitch;
     }
+  };
+  for (int t = t0; t < t1; t += kBatch) {
+    if (t + kBatch <= t1 && (!a.sequences || (t >= at.begin && t + kBatch <= at.end)))
+      batch(t, std::true_type());
+    else
+      batch(t, std::false_type());
   }
 }
 
@@ -164,48 +187,41 @@ __device__ void write_dstate(const lasp_conv_args& a, int row, int seq, int c) {
   const T* dy = static_cast<const T*>(a.dy.data) + (int64_t)row * a.dy.row_pitch + c;
   const int64_t at = (int64_t)seq * (W - 1) * a.channels + c;
   const T* from = a.state_in ? static_cast<const T*>(a.state_in) + at : nullptr;
+  constexpr int kPairs = Channels<V>::kPairs;
   Taps<T, V, W> taps;
   taps.load(a, c);
-  float bias[V], sum[W - 1][V];
-  load_bias<T, V>(a.bias, a.param_dtype, c, bias);
+  Channels<V> sum[W - 1];
 #pragma unroll
   for (int m = 0; m < W - 1; ++m) {
     const int kept = begin - end + m;   // its place in state_out, if it is there still
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[m][i] = 0.f;
-    if (a.dstate_out && kept >= 0) load_vec<T, V>(static_cast<const T*>(a.dstate_out) + at + (int64_t)kept * a.channels, sum[m]);
+    sum[m].clear();
+    if (a.dstate_out && kept >= 0) sum[m].load(static_cast<const T*>(a.dstate_out) + at + (int64_t)kept * a.channels);
   }
 #pragma unroll
   for (int r = 0; r < W - 1; ++r) {   // token begin + r reaches back to state entries r, r + 1, ...
     if (begin + r >= end) break;
-    float d[V], p[V];
-    load_vec<T, V>(dy + (int64_t)(begin + r) * a.dy.token_pitch, d);
+    Channels<V> d, past[W - 1];
+    d.load(dy + (int64_t)(begin + r) * a.dy.token_pitch);
     if (a.activation == LASP_ACT_SILU) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) p[i] = bias[i];
+      for (int m = 0; m < W - 1; ++m) past[m] = input_at<T, V, W>(x, a.x.token_pitch, from, a.channels, begin, begin + r - (W - 1) + m);
+      const Channels<V> now = input_at<T, V, W>(x, a.x.token_pitch, from, a.channels, begin, begin + r);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        float v[V];
-        input_at<T, V, W>(x, a.x.token_pitch, from, a.channels, begin, begin + r - (W - 1) + j, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = fmaf(taps.w[j][i], v[i], p[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) d[i] *= d_silu(p[i]);
+      for (int k = 0; k < kPairs; ++k) d.p[k] = mul2(d.p[k], d_silu(taps.sum(past, now.p[k], k)));
     }
 #pragma unroll
     for (int m = r; m < W - 1; ++m)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[m][i] = fmaf(taps.w[m - r][i], d[i], sum[m][i]);
+      for (int k = 0; k < kPairs; ++k) sum[m].p[k] = fma2(taps.w[m - r].p[k], d.p[k], sum[m].p[k]);
   }
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m) store_vec<T, V>(static_cast<T*>(a.dstate_in) + at + (int64_t)m * a.channels, sum[m]);
+  for (int m = 0; m < W - 1; ++m) sum[m].store(static_cast<T*>(a.dstate_in) + at + (int64_t)m * a.channels);
 }
 
 // partial: for each row and block of runs, W + 1 rows of `channels` sums (the taps' and the bias')
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(kVecs* kRuns) k_conv_backward(lasp_conv_args a, int run, int blocks_of_runs, float* partial) {
-  __shared__ float part[kRuns][kVecs * V];
+__global__ void __launch_bounds__(kVecs* kRuns, 4) k_conv_backward(lasp_conv_args a, int run, int blocks_of_runs, float* partial) {
+  __shared__ __align__(16) float part[kRuns][kVecs * V];
   const int c = (blockIdx.x * kVecs + threadIdx.x) * V, row = blockIdx.z;
   const bool mine = c < a.channels;
   if ((int)blockIdx.y >= blocks_of_runs) {
@@ -213,7 +229,10 @@ __global__ void __launch_bounds__(kVecs* kRuns) k_conv_backward(lasp_conv_args a
     if (mine && (a.sequences ? seq < a.sequences : threadIdx.y == 0)) write_dstate<T, V, W>(a, row, seq, c);
     return;
   }
-  float dw[W + 1][V] = {};
+  constexpr int kPairs = Channels<V>::kPairs;
+  Channels<V> dw[W + 1];
+#pragma unroll
+  for (int k = 0; k <= W; ++k) dw[k].clear();
   const int64_t first = ((int64_t)blockIdx.y * kRuns + threadIdx.y) * run;
   if (mine && first < a.tokens) {
     const int t0 = (int)first, t1 = first + run < a.tokens ? (int)first + run : a.tokens;
@@ -222,75 +241,70 @@ __global__ void __launch_bounds__(kVecs* kRuns) k_conv_backward(lasp_conv_args a
     T* dx = static_cast<T*>(a.dx.data) + (int64_t)row * a.dx.row_pitch + c;
     Taps<T, V, W> taps;
     taps.load(a, c);
-    float bias[V];
-    load_bias<T, V>(a.bias, a.param_dtype, c, bias);
+    // Token s completes dx_(s-W+1): a run stores those from its own first token's on, to which the W - 1 tokens ahead of it contribute; the
+    // row's last run completes the row.
+    const int ahead = t0 < W - 1 ? 0 : t0 - (W - 1);
     Place<T, W> at;
-    at.start(a, row, t0);
-    float past[W - 1][V], sum[W - 1][V];   // sum[m]: dx_(t-W+1+m) so far
+    at.start(a, row, ahead);
+    Channels<V> past[W - 1], sum[W - 1];   // sum[m]: dx_(t-W+1+m) so far
+    const auto look_back = [&](int t) {
 #pragma unroll
-    for (int m = 0; m < W - 1; ++m) {
-      input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, t0 - (W - 1) + m, past[m]);
+      for (int m = 0; m < W - 1; ++m)
+        past[m] = input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, t - (W - 1) + m);
+    };
+    look_back(ahead);
 #pragma unroll
-      for (int i = 0; i < V; ++i) sum[m][i] = 0.f;
-    }
-    // token t + W - 1 completes dx_t: a run looks W - 1 tokens beyond its end
-    const int stop = t1 + W - 1;
-    for (int t = t0; t < stop; t += kBatch) {
-      Vec<T, V> in[kBatch], din[kBatch];
+    for (int m = 0; m < W - 1; ++m) sum[m].clear();
+    // Tokens t to `stop`, kBatchBack at most.  `whole`: so many, in one sequence, W - 1 tokens or more behind its beginning, in this run
+    // and before what state_out holds.
+    const auto batch = [&](int t, int stop, auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      Vec<T, V> in[kBatchBack], din[kBatchBack];
+      const T *from = x + (int64_t)t * a.x.token_pitch, *dfrom = dy + (int64_t)t * a.dy.token_pitch;
+      T* to = dx + (int64_t)(t - (W - 1)) * a.dx.token_pitch;
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        if (t + j < stop && t + j < a.tokens) {
-          in[j] = *reinterpret_cast<const Vec<T, V>*>(x + (int64_t)(t + j) * a.x.token_pitch);
-          din[j] = *reinterpret_cast<const Vec<T, V>*>(dy + (int64_t)(t + j) * a.dy.token_pitch);
+      for (int j = 0; j < kBatchBack; ++j, from += a.x.token_pitch, dfrom += a.dy.token_pitch)
+        if (kWhole || (t + j < stop && t + j < a.tokens)) {
+          in[j] = *reinterpret_cast<const Vec<T, V>*>(from);
+          din[j] = *reinterpret_cast<const Vec<T, V>*>(dfrom);
         }
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
+      for (int j = 0; j < kBatchBack; ++j) {
         const int s = t + j;
-        if (s >= stop) break;
-        bool inside = s < a.tokens;
-        if (a.sequences && inside) {
+        if (!kWhole && s >= stop) break;
+        bool inside = kWhole || s < a.tokens;
+        if (!kWhole && a.sequences && inside) {
           if (s >= at.end) {
             at.advance(s);
-            if (s >= at.begin) {
-#pragma unroll
-              for (int m = 0; m < W - 1; ++m)
-                input_at<T, V, W>(x, a.x.token_pitch, at.state(a.state_in, a.channels, c), a.channels, at.begin, s - (W - 1) + m, past[m]);
-            }
+            if (s >= at.begin) look_back(s);
           }
           inside = at.inside(s);
         }
-        const int reach = inside ? s - at.begin : -1;   // how far back in its sequence this token's gradient goes
-        float out[V];
+        const int reach = kWhole ? W : inside ? s - at.begin : -1;   // how far back in its sequence this token's gradient goes
+        Channels<V> now, d, out;
+        now.set(in[j]), d.set(din[j]);
+        if (!inside) now.clear(), d.clear();
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float now = inside ? to_f(in[j].v[i]) : 0.f;
-          float d = inside ? to_f(din[j].v[i]) : 0.f;
-          if (a.activation == LASP_ACT_SILU) {
-            float p = fmaf(taps.w[W - 1][i], now, bias[i]);
+        for (int k = 0; k < kPairs; ++k) {
+          if (inside && a.activation == LASP_ACT_SILU) d.p[k] = mul2(d.p[k], d_silu(taps.sum(past, now.p[k], k)));
+          if (kWhole || (s >= t0 && inside)) {
 #pragma unroll
-            for (int m = 0; m < W - 1; ++m) p = fmaf(taps.w[m][i], past[m][i], p);
-            d = inside ? d * d_silu(p) : 0.f;
+            for (int m = 0; m < W - 1; ++m) dw[m].p[k] = fma2(d.p[k], past[m].p[k], dw[m].p[k]);
+            dw[W - 1].p[k] = fma2(d.p[k], now.p[k], dw[W - 1].p[k]);
+            dw[W].p[k] = add2(dw[W].p[k], d.p[k]);
           }
-          if (s < t1 && inside) {
+          F2 full[W];
 #pragma unroll
-            for (int m = 0; m < W - 1; ++m) dw[m][i] = fmaf(d, past[m][i], dw[m][i]);
-            dw[W - 1][i] = fmaf(d, now, dw[W - 1][i]);
-            dw[W][i] += d;
-          }
-          float full[W];
+          for (int m = 0; m < W - 1; ++m) full[m] = reach >= W - 1 - m ? fma2(taps.w[m].p[k], d.p[k], sum[m].p[k]) : sum[m].p[k];
+          full[W - 1] = mul2(taps.w[W - 1].p[k], d.p[k]);
+          out.p[k] = full[0];
 #pragma unroll
-          for (int m = 0; m < W - 1; ++m) full[m] = reach >= W - 1 - m ? fmaf(taps.w[m][i], d, sum[m][i]) : sum[m][i];
-          full[W - 1] = taps.w[W - 1][i] * d;
-          out[i] = full[0];
-#pragma unroll
-          for (int m = 0; m < W - 1; ++m) sum[m][i] = full[m + 1];
-#pragma unroll
-          for (int m = 0; m + 1 < W - 1; ++m) past[m][i] = past[m + 1][i];
-          past[W - 2][i] = now;
+          for (int m = 0; m < W - 1; ++m) sum[m].p[k] = full[m + 1];
         }
+        move_on(past, now);
         const int done = s - (W - 1);
-        if (done >= t0) {
-          if (a.dstate_out) {   // the last tokens of a sequence are in its state_out as well
+        if (kWhole || (s >= t0 && done >= 0)) {
+          if (!kWhole && a.dstate_out) {   // the last tokens of a sequence are in its state_out as well
             int seq = row, end = a.tokens;
             if (a.sequences) {
               int begin = 0;
@@ -299,28 +313,35 @@ __global__ void __launch_bounds__(kVecs* kRuns) k_conv_backward(lasp_conv_args a
             }
             const int kept = done - end + W - 1;
             if (seq >= 0 && done < end && kept >= 0) {
-              float more[V];
-              load_vec<T, V>(static_cast<const T*>(a.dstate_out) + ((int64_t)seq * (W - 1) + kept) * a.channels + c, more);
+              Channels<V> more;
+              more.load(static_cast<const T*>(a.dstate_out) + ((int64_t)seq * (W - 1) + kept) * a.channels + c);
 #pragma unroll
-              for (int i = 0; i < V; ++i) out[i] += more[i];
+              for (int k = 0; k < kPairs; ++k) out.p[k] = add2(out.p[k], more.p[k]);
             }
           }
-          store_vec<T, V>(dx + (int64_t)done * a.dx.token_pitch, out);
+          out.store(to);
         }
+        to += a.dx.token_pitch;
       }
+    };
+    if (ahead < t0) batch(ahead, t0, std::false_type());
+    for (int t = t0; t < t1; t += kBatchBack) {
+      if (t + kBatchBack <= t1 && t - at.begin >= W - 1 && t + kBatchBack <= at.end)
+        batch(t, t + kBatchBack, std::true_type());
+      else
+        batch(t, min(t + kBatchBack, t1), std::false_type());
     }
+    if (t1 == a.tokens) batch(t1, t1 + W - 1, std::false_type());
   }
   if (!partial) return;
   float* to = partial + ((int64_t)row * blocks_of_runs + blockIdx.y) * (W + 1) * a.channels;
   for (int k = 0; k <= W; ++k) {
     __syncthreads();
+    Channels<V> v = dw[0];   // (dw[k], with indexes that are known)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float v = dw[0][i];   // (dw[k], with indexes that are known)
-#pragma unroll
-      for (int q = 1; q <= W; ++q) v = k == q ? dw[q][i] : v;
-      part[threadIdx.y][threadIdx.x * V + i] = v;
-    }
+    for (int q = 1; q <= W; ++q)
+      if (k == q) v = dw[q];
+    v.store(&part[threadIdx.y][threadIdx.x * V]);
     __syncthreads();
     for (int e = threadIdx.y * kVecs + threadIdx.x; e < kVecs * V; e += kVecs * kRuns) {
       float s = 0.f;
@@ -361,44 +382,37 @@ __global__ void __launch_bounds__(128) k_conv_step(lasp_conv_step_args a) {
   const int64_t slot = a.slots ? index_at(a.slots, a.index_bits, row) : row;
   T* y = static_cast<T*>(a.y.data) + c;
   if (slot < 0 || slot >= a.slot_count) {   // a row that stands for no sequence
-    const float none[V] = {};
-    if (mine) store_vec<T, V>(y + (int64_t)row * a.y.row_pitch, none);
+    Channels<V> none;
+    none.clear();
+    if (mine) none.store(y + (int64_t)row * a.y.row_pitch);
     return;
   }
   const int shared = shared_slot(a.slots, a.index_bits, a.rows, row, slot);
   if (shared < 0 || !mine) return;
   T* state = static_cast<T*>(a.state) + slot * (W - 1) * a.channels + c;
-  const bool f32 = a.param_dtype == LASP_F32;
-  float past[W - 1][V], w[W][V], bias[V];
+  constexpr int kPairs = Channels<V>::kPairs;
+  Channels<V> past[W - 1];
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m) load_vec<T, V>(state + (int64_t)m * a.channels, past[m]);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = param<T>(a.weight, f32, (int64_t)(c + i) * W + j);
-  }
-  load_bias<T, V>(a.bias, a.param_dtype, c, bias);
+  for (int m = 0; m < W - 1; ++m) past[m].load(state + (int64_t)m * a.channels);
+  Taps<T, V, W> taps;
+  taps.load(a, c);
   for (int r = row; r < a.rows; ++r) {
-    if (r > row && (!shared || index_at(a.slots, a.index_bits, r) != slot)) {
+    if (r > row) {
       if (!shared) break;
-      continue;
+      if (index_at(a.slots, a.index_bits, r) != slot) continue;
     }
-    float now[V], out[V];
-    load_vec<T, V>(static_cast<const T*>(a.x.data) + (int64_t)r * a.x.row_pitch + c, now);
+    Channels<V> now, out;
+    now.load(static_cast<const T*>(a.x.data) + (int64_t)r * a.x.row_pitch + c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float p = fmaf(w[W - 1][i], now[i], bias[i]);
-#pragma unroll
-      for (int m = 0; m < W - 1; ++m) p = fmaf(w[m][i], past[m][i], p);
-      out[i] = a.activation == LASP_ACT_SILU ? silu(p) : p;
-#pragma unroll
-      for (int m = 0; m + 1 < W - 1; ++m) past[m][i] = past[m + 1][i];
-      past[W - 2][i] = now[i];
+    for (int k = 0; k < kPairs; ++k) {
+      const F2 p = taps.sum(past, now.p[k], k);
+      out.p[k] = a.activation == LASP_ACT_SILU ? silu(p) : p;
     }
-    store_vec<T, V>(y + (int64_t)r * a.y.row_pitch, out);
+    move_on(past, now);
+    out.store(y + (int64_t)r * a.y.row_pitch);
   }
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m) store_vec<T, V>(state + (int64_t)m * a.channels, past[m]);
+  for (int m = 0; m < W - 1; ++m) past[m].store(state + (int64_t)m * a.channels);
 }
 
 // Tokens of a run: long ones read fewer inputs twice and leave fewer partial sums, short ones give more threads.
@@ -412,13 +426,13 @@ int run_of(const lasp_conv_args& a, int v, int least) {
 }
 int blocks_of_runs(const lasp_conv_args& a, int run) { return (int)(((int64_t)a.tokens + (int64_t)run * kRuns - 1) / ((int64_t)run * kRuns)); }
 
+// V neighbouring channels of every tensor can be read and written by one access.
 template <typename T>
-bool wide(const lasp_conv_args& a, bool backward) {
-  constexpr int v = 16 / sizeof(T);
-  bool ok = a.channels % v == 0 && vector_ok(a.x, sizeof(T)) && vector_ok(a.state_in);
-  if (backward)
-    return ok && vector_ok(a.dy, sizeof(T)) && vector_ok(a.dx, sizeof(T)) && vector_ok(a.dstate_out) && vector_ok(a.dstate_in);
-  return ok && vector_ok(a.y, sizeof(T)) && vector_ok(a.state_out);
+bool wide(const lasp_conv_args& a, bool backward, int v) {
+  const auto tokens = [v](const lasp_tokens& t) { return by(t, v * sizeof(T), sizeof(T)); };
+  const auto states = [v](const void* p) { return reinterpret_cast<uintptr_t>(p) % (v * sizeof(T)) == 0; };
+  if (a.channels % v || !tokens(a.x) || !states(a.state_in)) return false;
+  return backward ? tokens(a.dy) && tokens(a.dx) && states(a.dstate_out) && states(a.dstate_in) : tokens(a.y) && states(a.state_out);
 }
 
 template <typename T, int V, int W>
@@ -451,11 +465,13 @@ cudaError_t backward_of(const lasp_conv_args& a, cudaStream_t st) {
   return a.width == 4 ? backward_as<T, V, 4>(a, st) : a.width == 3 ? backward_as<T, V, 3>(a, st) : backward_as<T, V, 2>(a, st);
 }
 
+// Channels of a thread.  Eight need 250 registers: 8 x 2048 x 4096 bf16 took 177 us forward and 552 backward, four 76 and 179, a pair (packed
+// arithmetic, five and four blocks an SM) 66 and 131.
+constexpr int kPair = 2;
 template <typename T>
 cudaError_t dispatch(const lasp_conv_args& a, bool backward, cudaStream_t st) {
-  constexpr int v = 16 / sizeof(T);
-  if (wide<T>(a, backward)) return backward ? backward_of<T, v>(a, st) : forward_of<T, v>(a, st);
-  return backward ? backward_of<T, 1>(a, st) : forward_of<T, 1>(a, st);
+  if (backward) return wide<T>(a, true, kPair) ? backward_of<T, kPair>(a, st) : backward_of<T, 1>(a, st);
+  return wide<T>(a, false, kPair) ? forward_of<T, kPair>(a, st) : forward_of<T, 1>(a, st);
 }
 
 template <typename T, int V>
@@ -472,7 +488,7 @@ cudaError_t step_of(const lasp_conv_step_args& a, cudaStream_t st) {
 template <typename T>
 cudaError_t step_as(const lasp_conv_step_args& a, cudaStream_t st) {
   constexpr int v = 16 / sizeof(T);
-  const bool ok = a.channels % v == 0 && vector_ok(a.x, sizeof(T)) && vector_ok(a.y, sizeof(T)) && vector_ok(a.state);
+  const bool ok = a.channels % v == 0 && by(a.x, 16, sizeof(T)) && by(a.y, 16, sizeof(T)) && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
   return ok ? step_of<T, v>(a, st) : step_of<T, 1>(a, st);
 }
 
@@ -486,8 +502,7 @@ cudaError_t conv_backward(const lasp_conv_args& a, cudaStream_t st) {
 }
 // (for either width of the accesses: it must not depend on the addresses, which the caller may not have yet)
 size_t conv_workspace(const lasp_conv_args& a) {
-  const int v = a.dtype == LASP_F32 ? 4 : 8;
-  const int blocks = std::max(blocks_of_runs(a, run_of(a, v, 4 * kBatch)), blocks_of_runs(a, run_of(a, 1, 4 * kBatch)));
+  const int blocks = std::max(blocks_of_runs(a, run_of(a, kPair, 4 * kBatch)), blocks_of_runs(a, run_of(a, 1, 4 * kBatch)));
   return (size_t)a.rows * blocks * (a.width + 1) * a.channels * sizeof(float);
 }
 cudaError_t conv_step(const lasp_conv_step_args& a, cudaStream_t st) {

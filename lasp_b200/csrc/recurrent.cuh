@@ -1,5 +1,9 @@
 // Shared by the recurrences over tokens (conv_kernels.cu, scan_*.cu): types, sequences of a batch, rows that share a slot.
 #pragma once
+#include <string.h>
+
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lasp {
@@ -39,20 +43,141 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
-template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&out)[V]) {
-  const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = to_f(x.v[i]);
+// Arithmetic on pairs, one instruction for two fp32 values.  A pair is kept as the 64 bits that those instructions take: taken apart
+// and put together again it would cost a move each time (a third of all instructions, when it was).
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void apart(F2 p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
+// Two neighbouring 16-bit numbers are a word, which is taken apart and put together whole (two instructions and one).
+template <typename T>
+__device__ __forceinline__ F2 pair_from(const T* two) {
+  if constexpr (sizeof(T) == 4) {
+    return f2(two[0], two[1]);
+  } else {
+    uint32_t w;
+    memcpy(&w, two, 4);
+    if constexpr (std::is_same<T, __half>::value) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      return f2(v.x, v.y);
+    } else {
+      return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void pair_to(T* two, float x, float y) {
+  if constexpr (sizeof(T) == 4) {
+    two[0] = x, two[1] = y;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(x, y);
+    memcpy(two, &v, 4);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    memcpy(two, &v, 4);
+  }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
   Vec<T, V> x;
+  if constexpr (V % 2) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) x.v[i] = from_f<T>(in[i]);
+    for (int i = 0; i < V; ++i) x.v[i] = from_f<T>(in[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pair_to(&x.v[i], in[i], in[i + 1]);
+  }
   *reinterpret_cast<Vec<T, V>*>(p) = x;
 }
 
+// x sigmoid(x) and its derivative; 1 / (1 + e^-x) by the fast exponential and reciprocal (2^-21 relative, where the result is
+// rounded to fp32's 2^-24 at best): an infinite e^-x gives 0.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid(float x) { return reciprocal(1.f + ex2(-kLog2e * x)); }
+__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+__device__ __forceinline__ float d_silu(float x) {
+  const float s = sigmoid(x);
+  return s + x * s * (1.f - s);
+}
+
+__device__ __forceinline__ F2 sigmoid(F2 p) {
+  float x, y;
+  apart(mul2(p, f2(-kLog2e, -kLog2e)), x, y);
+  apart(add2(f2(ex2(x), ex2(y)), f2(1.f, 1.f)), x, y);
+  return f2(reciprocal(x), reciprocal(y));
+}
+__device__ __forceinline__ F2 silu(F2 p) { return mul2(p, sigmoid(p)); }
+__device__ __forceinline__ F2 d_silu(F2 p) {   // s + p s (1 - s) = s (1 + p) - (s p) s
+  const F2 s = sigmoid(p), sp = mul2(s, p);
+  return fma2(mul2(sp, f2(-1.f, -1.f)), s, add2(s, sp));
+}
+
+// V neighbouring channels as pairs; of a single channel the other half is zero.
+template <int V>
+struct Channels {
+  static constexpr int kPairs = (V + 1) / 2;
+  F2 p[kPairs];
+  template <typename T>
+  __device__ __forceinline__ void set(const Vec<T, V>& x) {
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k)
+      if constexpr (V > 1)
+        p[k] = pair_from(&x.v[2 * k]);
+      else
+        p[k] = f2(to_f(x.v[0]), 0.f);
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* from) { set(*reinterpret_cast<const Vec<T, V>*>(from)); }
+  template <typename T>
+  __device__ __forceinline__ void store(T* to) const {
+    Vec<T, V> v;
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) {
+      float x, y;
+      apart(p[k], x, y);
+      if constexpr (V > 1)
+        pair_to(&v.v[2 * k], x, y);
+      else
+        v.v[0] = from_f<T>(x);
+    }
+    *reinterpret_cast<Vec<T, V>*>(to) = v;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) p[k] = f2(0.f, 0.f);
+  }
+};
 __device__ __forceinline__ int64_t index_at(const void* p, int bits, int64_t i) {
   return bits == 64 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
 }
@@ -96,19 +221,11 @@ __device__ __forceinline__ int shared_slot(const void* slots, int bits, int rows
   return before ? -1 : after;
 }
 
-// x sigmoid(x) and its derivative; 1 / (1 + e^-x) by the fast exponential and division (2^-21 relative, where the result is
-// rounded to fp32's 2^-24 at best): an infinite e^-x gives 0.
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
-__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
-__device__ __forceinline__ float d_silu(float x) {
-  const float s = sigmoid(x);
-  return s + x * s * (1.f - s);
+// A tensor of tokens can be read and written by `bytes` at a time.
+inline bool by(const lasp_tokens& t, size_t bytes, size_t item) {
+  const uint64_t at = reinterpret_cast<uintptr_t>(t.data) | (uint64_t)t.row_pitch * item | (uint64_t)t.token_pitch * item | (uint64_t)t.group_pitch * item;
+  return !t.data || (at & (bytes - 1)) == 0;
 }
-
-inline bool vector_ok(const lasp_tokens& t, size_t item) {
-  return !t.data || ((reinterpret_cast<uintptr_t>(t.data) | (size_t)(t.row_pitch * (int64_t)item) | (size_t)(t.token_pitch * (int64_t)item)) & 15) == 0;
-}
-inline bool vector_ok(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 cudaError_t conv_forward(const lasp_conv_args& a, cudaStream_t st);
 cudaError_t conv_backward(const lasp_conv_args& a, cudaStream_t st);

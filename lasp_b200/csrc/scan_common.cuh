@@ -14,8 +14,6 @@
 
 namespace lasp {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
 constexpr int kChunk = 16, kGroup = 128, kThreads = 3 * kGroup;   // warps come in groups of four
 template <int LPC>
 struct Tile {
@@ -81,34 +79,7 @@ template <typename T, int N>
 __device__ __forceinline__ void numbers(const Vec<T, N>& from, float (&out)[N]) {
   const Vec<T, N> v = from;
 #pragma unroll
-  for (int k = 0; k < N; ++k) out[k] = to_f(v.v[k]);
-}
-
-// Arithmetic on pairs, one instruction for two fp32 values.  A pair is kept as the 64 bits that those instructions take: taken apart
-// and put together again it would cost a move each time (a third of all instructions, when it was).
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void apart(F2 p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
+  for (int k = 0; k < N; k += 2) apart(pair_from(&v.v[k]), out[k], out[k + 1]);
 }
 
 // 4 states
@@ -132,11 +103,6 @@ __device__ __forceinline__ S4 load4(const void* p) {   // 16 aligned bytes
 }
 __device__ __forceinline__ F2 pair_of(const void* p) { return {*static_cast<const unsigned long long*>(p)}; }   // 8 aligned bytes
 __device__ __forceinline__ void store4(void* p, S4 s) { *static_cast<ulonglong2*>(p) = make_ulonglong2(s.a.v, s.b.v); }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ F2 exp2(F2 p) {
   float x, y;
   apart(p, x, y);
@@ -180,7 +146,7 @@ __device__ __forceinline__ F2 softplus(F2 p) {
   float x, y;
   apart(p, x, y);
   const float ex = ex2(-fabsf(x) * kLog2e), ey = ex2(-fabsf(y) * kLog2e);
-  const F2 s = f2(__fdividef(ex, 2.f + ex), __fdividef(ey, 2.f + ey)), q = mul2(s, s);
+  const F2 s = f2(ex * reciprocal(2.f + ex), ey * reciprocal(2.f + ey)), q = mul2(s, s);
   const auto k = [](float c) { return f2(c, c); };
   F2 t = fma2(q, k(1.f / 13), k(1.f / 11));
   t = fma2(q, t, k(1.f / 9)), t = fma2(q, t, k(1.f / 7)), t = fma2(q, t, k(1.f / 5)), t = fma2(q, t, k(1.f / 3));
@@ -250,12 +216,9 @@ __device__ __forceinline__ Stretch stretch_of(const lasp_scan_args& a, int seq) 
 inline int64_t chunks_of(const lasp_scan_args& a) {
   return a.sequences ? (int64_t)a.tokens / kChunk + a.sequences + 1 : (int64_t)a.rows * ((a.tokens + kChunk - 1) / kChunk);
 }
-// n neighbouring numbers (n * sizeof(T) <= 16, or a multiple of 16) of a tensor of tokens can be read and written by one access.
+// n neighbouring numbers of a tensor of tokens can be read and written by accesses of all their bytes, or of 16.
 template <typename T>
-bool reads_by(const lasp_tokens& t, int n) {
-  const int bytes = std::min<int>(16, n * (int)sizeof(T)), items = bytes / (int)sizeof(T);
-  return !t.data || (reinterpret_cast<uintptr_t>(t.data) % bytes == 0 && t.row_pitch % items == 0 && t.token_pitch % items == 0 && t.group_pitch % items == 0);
-}
+bool reads_by(const lasp_tokens& t, int n) { return by(t, std::min<size_t>(16, n * sizeof(T)), sizeof(T)); }
 inline int padded_states(int states) { return states <= 16 ? 16 : states <= 32 ? 32 : 64; }
 
 template <typename T, int N>
