@@ -375,44 +375,60 @@ __global__ void __launch_bounds__(256) k_conv_params(lasp_conv_args a, const flo
   }
 }
 
+// Single tokens: the inputs before the next row's token, and that token, are sent for before this row is worked on.
+constexpr int kStepThreads = 128;
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(128) k_conv_step(lasp_conv_step_args a) {
-  const int row = blockIdx.y, c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
+__global__ void __launch_bounds__(kStepThreads) k_conv_step(lasp_conv_step_args a, int per) {
+  __shared__ StepRows rows;
+  const int row0 = blockIdx.y * per, count = min(per, a.rows - row0), c = (blockIdx.x * kStepThreads + threadIdx.x) * V;
   const bool mine = c < a.channels;
-  const int64_t slot = a.slots ? index_at(a.slots, a.index_bits, row) : row;
-  T* y = static_cast<T*>(a.y.data) + c;
-  if (slot < 0 || slot >= a.slot_count) {   // a row that stands for no sequence
-    Channels<V> none;
-    none.clear();
-    if (mine) none.store(y + (int64_t)row * a.y.row_pitch);
-    return;
-  }
-  const int shared = shared_slot(a.slots, a.index_bits, a.rows, row, slot);
-  if (shared < 0 || !mine) return;
-  T* state = static_cast<T*>(a.state) + slot * (W - 1) * a.channels + c;
+  const auto state = [&](int64_t slot) { return static_cast<T*>(a.state) + slot * (W - 1) * a.channels + c; };
   constexpr int kPairs = Channels<V>::kPairs;
-  Channels<V> past[W - 1];
+  Channels<V> next[W - 1], x;
+  const auto token = [&](int r) { return static_cast<const T*>(a.x.data) + (int64_t)r * a.x.row_pitch + c; };
+  const auto fetch = [&](int r, int64_t slot) {
+    if (slot < 0 || slot >= a.slot_count || !mine) return;
 #pragma unroll
-  for (int m = 0; m < W - 1; ++m) past[m].load(state + (int64_t)m * a.channels);
+    for (int m = 0; m < W - 1; ++m) next[m].load(state(slot) + (int64_t)m * a.channels);
+    x.load(token(r));
+  };
+  fetch(row0, a.slots ? index_at(a.slots, a.index_bits, row0) : row0);
   Taps<T, V, W> taps;
-  taps.load(a, c);
-  for (int r = row; r < a.rows; ++r) {
-    if (r > row) {
-      if (!shared) break;
-      if (index_at(a.slots, a.index_bits, r) != slot) continue;
-    }
-    Channels<V> now, out;
-    now.load(static_cast<const T*>(a.x.data) + (int64_t)r * a.x.row_pitch + c);
+  if (mine) taps.load(a, c);
+  rows.find(a.slots, a.index_bits, a.rows, row0, count);
+  if (!mine) return;
+  for (int q = 0; q < count; ++q) {
+    const int64_t slot = rows.slot[q];
+    Channels<V> past[W - 1], now = x;
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) {
-      const F2 p = taps.sum(past, now.p[k], k);
-      out.p[k] = a.activation == LASP_ACT_SILU ? silu(p) : p;
+    for (int m = 0; m < W - 1; ++m) past[m] = next[m];
+    if (q + 1 < count && rows.first(q + 1)) fetch(row0 + q + 1, rows.slot[q + 1]);
+    T* y = static_cast<T*>(a.y.data) + c;
+    if (slot < 0 || slot >= a.slot_count) {   // a row that stands for no sequence
+      Channels<V> none;
+      none.clear();
+      none.store(y + (int64_t)(row0 + q) * a.y.row_pitch);
+      continue;
     }
-    move_on(past, now);
-    out.store(y + (int64_t)r * a.y.row_pitch);
+    if (!rows.first(q)) continue;
+    for (int r = row0 + q; r < a.rows; ++r) {
+      if (r > row0 + q) {
+        if (!rows.shared(q)) break;
+        if (index_at(a.slots, a.index_bits, r) != slot) continue;
+        now.load(token(r));
+      }
+      Channels<V> out;
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const F2 p = taps.sum(past, now.p[k], k);
+        out.p[k] = a.activation == LASP_ACT_SILU ? silu(p) : p;
+      }
+      move_on(past, now);
+      out.store(y + (int64_t)r * a.y.row_pitch);
+    }
+#pragma unroll
+    for (int m = 0; m < W - 1; ++m) past[m].store(state(slot) + (int64_t)m * a.channels);
   }
-#pragma unroll
-  for (int m = 0; m < W - 1; ++m) past[m].store(state + (int64_t)m * a.channels);
 }
 
 // Tokens of a run: long ones read fewer inputs twice and leave fewer partial sums, short ones give more threads.
@@ -476,19 +492,21 @@ cudaError_t dispatch(const lasp_conv_args& a, bool backward, cudaStream_t st) {
 
 template <typename T, int V>
 cudaError_t step_of(const lasp_conv_step_args& a, cudaStream_t st) {
-  const dim3 grid((a.channels + 128 * V - 1) / (128 * V), a.rows);
+  const int tiles = (a.channels + kStepThreads * V - 1) / (kStepThreads * V), per = step_rows(a.rows, tiles, 8);
+  const dim3 grid(tiles, (a.rows + per - 1) / per);
   if (a.width == 4)
-    k_conv_step<T, V, 4><<<grid, 128, 0, st>>>(a);
+    k_conv_step<T, V, 4><<<grid, kStepThreads, 0, st>>>(a, per);
   else if (a.width == 3)
-    k_conv_step<T, V, 3><<<grid, 128, 0, st>>>(a);
+    k_conv_step<T, V, 3><<<grid, kStepThreads, 0, st>>>(a, per);
   else
-    k_conv_step<T, V, 2><<<grid, 128, 0, st>>>(a);
+    k_conv_step<T, V, 2><<<grid, kStepThreads, 0, st>>>(a, per);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t step_as(const lasp_conv_step_args& a, cudaStream_t st) {
-  constexpr int v = 16 / sizeof(T);
-  const bool ok = a.channels % v == 0 && by(a.x, 16, sizeof(T)) && by(a.y, 16, sizeof(T)) && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
+  constexpr int v = 4;
+  const auto fits = [](const lasp_tokens& t) { return by(t, v * sizeof(T), sizeof(T)); };
+  const bool ok = a.channels % v == 0 && fits(a.x) && fits(a.y) && reinterpret_cast<uintptr_t>(a.state) % (v * sizeof(T)) == 0;
   return ok ? step_of<T, v>(a, st) : step_of<T, 1>(a, st);
 }
 

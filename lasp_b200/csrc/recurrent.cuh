@@ -209,16 +209,32 @@ struct Sequences {
   }
 };
 
-// Rows of a step that name the same slot are consecutive tokens: the first of them takes the others along.  Every thread of the
-// block calls this.  Returns -1 where an earlier row has the slot, 1 where a later one has, else 0.
-__device__ __forceinline__ int shared_slot(const void* slots, int bits, int rows, int row, int64_t slot) {
-  if (!slots || rows == 1) return 0;
-  int before = 0, after = 0;
-  for (int j = threadIdx.x + threadIdx.y * blockDim.x; j < rows; j += blockDim.x * blockDim.y)
-    if (j != row && index_at(slots, bits, j) == slot) (j < row ? before : after) = 1;
-  before = __syncthreads_or(before);
-  after = __syncthreads_or(after);
-  return before ? -1 : after;
+// Single tokens: a block takes some channels of kStepRows rows at most, so that what belongs to the channels is read once.  Rows that name
+// the same slot are consecutive tokens: the first of them takes the others along.
+constexpr int kStepRows = 32;
+struct StepRows {
+  int64_t slot[kStepRows];
+  uint32_t before, after;   // a bit for each row: an earlier, a later row has its slot
+  __device__ __forceinline__ bool first(int q) const { return !(before >> q & 1); }
+  __device__ __forceinline__ bool shared(int q) const { return after >> q & 1; }
+  // (every thread of the block calls it; the block has at least kStepRows)
+  __device__ __forceinline__ void find(const void* slots, int bits, int rows, int row0, int n) {
+    if (threadIdx.x == 0) before = after = 0;
+    if (threadIdx.x < n) slot[threadIdx.x] = slots ? index_at(slots, bits, row0 + threadIdx.x) : row0 + threadIdx.x;
+    __syncthreads();
+    if (!slots || rows == 1) return;
+    for (int j = threadIdx.x; j < rows; j += blockDim.x) {
+      const int64_t s = index_at(slots, bits, j);
+      for (int q = 0; q < n; ++q)
+        if (s == slot[q] && j != row0 + q) atomicOr(j < row0 + q ? &before : &after, 1u << q);
+    }
+    __syncthreads();
+  }
+};
+// Rows of a block: as few as leave no more than `resident` blocks for each SM, all of them at work at once.
+inline int step_rows(int rows, int tiles, int resident) {
+  const int64_t blocks = std::max<int64_t>(1, (int64_t)resident * sm_count() / tiles);   // for the rows
+  return (int)std::min<int64_t>(kStepRows, (rows + blocks - 1) / blocks);
 }
 
 // A tensor of tokens can be read and written by `bytes` at a time.

@@ -178,7 +178,7 @@ __device__ __forceinline__ void store_four(float* p, int n, int states, float4 v
 // keeps the state
 __device__ __forceinline__ S4 rates(const float* A, int n, int states) {
   const float4 v = four_of(A, n, states);
-  const auto one = [](float x) { return isinf(x) ? copysignf(3.402823466e38f, x) : x * kLog2e; };
+  const auto one = [](float x) { return x *= kLog2e, isinf(x) ? copysignf(3.402823466e38f, x) : x; };
   return {f2(one(v.x), one(v.y)), f2(one(v.z), one(v.w))};
 }
 

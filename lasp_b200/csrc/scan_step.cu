@@ -5,89 +5,134 @@
 namespace lasp {
 namespace {
 
-constexpr int kStepThreads = 128, kOwn = 4;   // channels of a lane, side by side: that many reads of the state under way
+constexpr int kStepThreads = 128, kStepBlocks = 5;   // (blocks: of an SM)
+constexpr int kOwn = 4;                              // channels of a lane, side by side: that many reads of the state under way
 
-// A lane holds 4 states of each of its channels; LPC lanes side by side have those of a channel.  wide: u, dt, B and C can be read by four.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(kStepThreads) k_scan_step(lasp_scan_step_args a, bool wide) {
-  constexpr int kSame = LPC / kOwn;   // lanes that are left with the same channel's sum
-  const int row = blockIdx.y, lane = threadIdx.x % 32, i = threadIdx.x % LPC, n = 4 * i;
-  const int c0 = (blockIdx.x * (kStepThreads / LPC) + threadIdx.x / LPC) * kOwn, mine = c0 + i / kSame;   // mine: whose output this lane finishes
-  const bool f32 = a.param_dtype == LASP_F32, writes = i % kSame == 0 && mine < a.channels;
-  const int64_t slot = a.slots ? index_at(a.slots, a.index_bits, row) : row;
-  if (slot < 0 || slot >= a.slot_count) {   // a row that stands for no sequence
-    if (writes) static_cast<T*>(a.y.data)[(int64_t)row * a.y.row_pitch + mine] = from_f<T>(0.f);
-    return;
-  }
-  float* state = a.state + (slot * a.channels + c0) * a.states;
-  const float* A = a.A + (int64_t)c0 * a.states;
-  const int left = a.channels - c0;
-  S4 h[kOwn], rate[kOwn];
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) h[k] = k < left ? s4(four_of(state + (int64_t)k * a.states, n, a.states)) : splat(0.f);
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) rate[k] = k < left ? rates(A + (int64_t)k * a.states, n, a.states) : splat(0.f);
-  const int shared = shared_slot(a.slots, a.index_bits, a.rows, row, slot);   // (the state is on its way meanwhile)
-  if (shared < 0) return;
-  float bias[kOwn];
-#pragma unroll
-  for (int k = 0; k < kOwn; ++k) bias[k] = k < left && a.dt_bias ? param<T>(a.dt_bias, f32, c0 + k) : 0.f;
-  const float skip = writes && a.D ? param<T>(a.D, f32, mine) : 0.f;
-  const int in_group = a.channels / a.groups, group = (c0 < a.channels ? c0 : 0) / in_group;
-  const bool one_group = left >= kOwn && (c0 + kOwn - 1) / in_group == group;
-  for (int r = row; r < a.rows; ++r) {
-    if (r > row) {
-      if (!shared) break;
-      if (index_at(a.slots, a.index_bits, r) != slot) continue;
-    }
-    const auto rows = [&](const lasp_tokens& t) { return static_cast<T*>(t.data) + (int64_t)r * t.row_pitch; };
-    const auto four = [&](const lasp_tokens& t, int g) {   // this lane's states of B or C
-      const T* p = rows(t) + (int64_t)g * t.group_pitch + n;
-      float x[4] = {};
-      if (wide && n + 4 <= a.states) {
-        numbers<T, 4>(*reinterpret_cast<const Vec<T, 4>*>(p), x);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (n + q < a.states) x[q] = to_f(p[q]);
-      }
-      return s4(make_float4(x[0], x[1], x[2], x[3]));
-    };
-    float u[kOwn] = {}, dt[kOwn] = {}, y[kOwn];
-    if (wide && left >= kOwn) {
-      numbers<T, kOwn>(*reinterpret_cast<const Vec<T, kOwn>*>(rows(a.u) + c0), u), numbers<T, kOwn>(*reinterpret_cast<const Vec<T, kOwn>*>(rows(a.dt) + c0), dt);
+// A lane holds 4 states of each of its channels; LPC lanes side by side have those of a channel.  The state of the next row is sent for
+// before this one's is worked on.  What belongs to a channel and token (step, input, gate) is worked out by one lane and handed round.
+// WHOLE: every lane has four states of four channels of one group, reads the states, B and C by four, and numbers and pitches have 32
+// bits; checks for less than that and 64-bit products were half of all instructions.
+template <typename T, int LPC, bool WHOLE>
+__global__ void __launch_bounds__(kStepThreads, kStepBlocks) k_scan_step(lasp_scan_step_args a, int per) {
+  __shared__ StepRows rows;
+  constexpr int kSame = LPC / kOwn;   // lanes that work on the same channel
+  const int lane = threadIdx.x % 32, i = threadIdx.x % LPC, n = 4 * i, row0 = blockIdx.y * per, count = min(per, a.rows - row0);
+  const int c0 = (blockIdx.x * (kStepThreads / LPC) + threadIdx.x / LPC) * kOwn, mine = c0 + i / kSame, length = WHOLE ? 4 * LPC : a.states;
+  const int own = WHOLE ? (c0 < a.channels ? kOwn : 0) : min(kOwn, a.channels - c0);
+  const bool f32 = a.param_dtype == LASP_F32, there = mine < a.channels, writes = there && i % kSame == 0;
+  const int64_t pitch = (int64_t)a.channels * length;
+  float* const state = a.state + (int64_t)c0 * length;
+  const auto by_slot = [&](int64_t slot) { return WHOLE ? (uint64_t)(uint32_t)pitch * (uint32_t)slot : (uint64_t)(slot * pitch); };
+  const auto get = [&](const float* p) { return WHOLE ? *reinterpret_cast<const float4*>(p + n) : four_of(p, n, length); };
+  const int in_group = a.channels / a.groups, group = (own > 0 ? c0 : 0) / in_group;
+  // row r of a tensor, from a place in its first row
+  const auto at = [&](T* p, int64_t row_pitch, int r) {
+    return WHOLE ? p + (uint64_t)(uint32_t)row_pitch * (uint32_t)r : p + row_pitch * r;
+  };
+  T *const pu = static_cast<T*>(a.u.data) + mine, *const pdt = static_cast<T*>(a.dt.data) + mine, *const pz = static_cast<T*>(a.z.data) + mine;
+  T *const py = static_cast<T*>(a.y.data) + mine, *const pB = static_cast<T*>(a.B.data) + n, *const pC = static_cast<T*>(a.C.data) + n;
+  T *const gB = pB + group * a.B.group_pitch, *const gC = pC + group * a.C.group_pitch;
+  const auto four = [&](const T* p) {   // this lane's states of B or C
+    if constexpr (WHOLE) {
+      return *reinterpret_cast<const Vec<T, 4>*>(p);
     } else {
+      Vec<T, 4> x;
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k)
-        if (k < left) u[k] = to_f(rows(a.u)[c0 + k]), dt[k] = to_f(rows(a.dt)[c0 + k]);
+      for (int m = 0; m < 4; ++m) x.v[m] = n + m < length ? p[m] : from_f<T>(0.f);
+      return x;
     }
-    S4 B = four(a.B, group), C = four(a.C, group);
+  };
+  S4 h[kOwn], rate[kOwn], next[kOwn];
+  Vec<T, 4> next_B, next_C;
+  T next_u = from_f<T>(0.f), next_dt = next_u, next_z = next_u;
+  const auto fetch_token = [&](int r) {
+    next_B = four(at(gB, a.B.row_pitch, r)), next_C = four(at(gC, a.C.row_pitch, r));
+    if (there) next_u = *at(pu, a.u.row_pitch, r), next_dt = *at(pdt, a.dt.row_pitch, r);
+    if (there && a.z.data) next_z = *at(pz, a.z.row_pitch, r);
+  };
+  const auto fetch = [&](int r, int64_t slot) {
+    if (slot < 0 || slot >= a.slot_count) return;
+    const float* from = state + by_slot(slot);
 #pragma unroll
-    for (int k = 0; k < kOwn; ++k) {
-      if (!one_group && k && k < left) B = four(a.B, (c0 + k) / in_group), C = four(a.C, (c0 + k) / in_group);
-      float step = dt[k] + bias[k];
-      if (a.softplus) step = softplus(step);
-      const float in = step * u[k];
-      h[k] = fma(exp2(mul(rate[k], f2(step, step))), h[k], mul(B, f2(in, in)));
-      y[k] = dot(h[k], C);
-    }
-    sum_over<kOwn, LPC, 1>(y, lane);
-    if (writes) {
-      float out = a.D ? fmaf(skip, to_f(rows(a.u)[mine]), y[0]) : y[0];
-      if (a.z.data) out *= silu(to_f(rows(a.z)[mine]));
-      rows(a.y)[mine] = from_f<T>(out);
-    }
-  }
+    for (int k = 0; k < kOwn; ++k)
+      if (k < own) next[k] = s4(get(from + k * length));
+    fetch_token(r);
+  };
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) next[k] = rate[k] = splat(0.f);
+  fetch(row0, a.slots ? index_at(a.slots, a.index_bits, row0) : row0);
 #pragma unroll
   for (int k = 0; k < kOwn; ++k)
-    if (k < left) store_four(state + (int64_t)k * a.states, n, a.states, f4(h[k]));
+    if (k < own) rate[k] = rates(a.A + (int64_t)(c0 + k) * length, n, length);
+  const float bias = there && a.dt_bias ? param<T>(a.dt_bias, f32, mine) : 0.f, skip = there && a.D ? param<T>(a.D, f32, mine) : 0.f;
+  rows.find(a.slots, a.index_bits, a.rows, row0, count);
+  for (int q = 0; q < count; ++q) {
+    const int64_t slot = rows.slot[q];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) h[k] = next[k];
+    Vec<T, 4> now_B = next_B, now_C = next_C;
+    T now_u = next_u, now_dt = next_dt, now_z = next_z;
+    const bool more = q + 1 < count && rows.first(q + 1);
+    if (more) fetch(row0 + q + 1, rows.slot[q + 1]);
+    if (slot < 0 || slot >= a.slot_count) {   // a row that stands for no sequence
+      if (writes) *at(py, a.y.row_pitch, row0 + q) = from_f<T>(0.f);
+      continue;
+    }
+    if (!rows.first(q)) continue;
+    for (int r = row0 + q; r < a.rows; ++r) {
+      if (r > row0 + q) {
+        if (!rows.shared(q)) break;
+        if (index_at(a.slots, a.index_bits, r) != slot) continue;
+        now_B = four(at(gB, a.B.row_pitch, r)), now_C = four(at(gC, a.C.row_pitch, r));
+        if (there) now_u = *at(pu, a.u.row_pitch, r), now_dt = *at(pdt, a.dt.row_pitch, r);
+        if (there && a.z.data) now_z = *at(pz, a.z.row_pitch, r);
+      }
+      const auto s4_of = [](const Vec<T, 4>& v) { return S4{pair_from(&v.v[0]), pair_from(&v.v[2])}; };
+      S4 B = s4_of(now_B), C = s4_of(now_C);
+      const float u = to_f(now_u);
+      float step = to_f(now_dt) + bias, y[kOwn];
+      if (a.softplus) step = softplus(step);
+      const float in = step * u;
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        const float dt = __shfl_sync(~0u, step, k * kSame, LPC), x = __shfl_sync(~0u, in, k * kSame, LPC);
+        if constexpr (!WHOLE)
+          if (const int64_t g = (c0 + k) / in_group; k && k < own && (c0 + k) % in_group == 0)
+            B = s4_of(four(at(pB + g * a.B.group_pitch, a.B.row_pitch, r))), C = s4_of(four(at(pC + g * a.C.group_pitch, a.C.row_pitch, r)));
+        h[k] = fma(exp2(mul(rate[k], f2(dt, dt))), h[k], mul(B, f2(x, x)));
+        y[k] = dot(h[k], C);
+      }
+      sum_over<kOwn, LPC, 1>(y, lane);
+      if (a.D) y[0] = fmaf(skip, u, y[0]);
+      if (a.z.data) y[0] *= silu(to_f(now_z));
+      if (writes) *at(py, a.y.row_pitch, r) = from_f<T>(y[0]);
+    }
+    float* to = state + by_slot(slot);
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      if (k < own) {
+        if constexpr (WHOLE)
+          store4(to + k * length + n, h[k]);
+        else
+          store_four(to + k * length, n, length, f4(h[k]));
+      }
+  }
 }
 
 template <typename T, int LPC>
 cudaError_t launch(const lasp_scan_step_args& a, cudaStream_t st) {
   constexpr int channels = kStepThreads / LPC * kOwn;
-  const bool wide = reads_by<T>(a.u, kOwn) && reads_by<T>(a.dt, kOwn) && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
-  k_scan_step<T, LPC><<<dim3((a.channels + channels - 1) / channels, a.rows), kStepThreads, 0, st>>>(a, wide);
+  const auto small = [](int64_t n) { return n >= 0 && n <= INT32_MAX; };
+  bool whole = small(a.slot_count) && small((int64_t)a.channels * a.states);
+  for (const lasp_tokens* t : {&a.u, &a.dt, &a.z, &a.B, &a.C, &a.y}) whole = whole && small(t->row_pitch);
+  whole = whole && a.states == 4 * LPC && a.channels / a.groups % kOwn == 0 && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4) &&
+          (reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.A)) % 16 == 0;
+  const int tiles = (a.channels + channels - 1) / channels, per = step_rows(a.rows, tiles, kStepBlocks);
+  const dim3 grid(tiles, (a.rows + per - 1) / per);
+  if (whole)
+    k_scan_step<T, LPC, true><<<grid, kStepThreads, 0, st>>>(a, per);
+  else
+    k_scan_step<T, LPC, false><<<grid, kStepThreads, 0, st>>>(a, per);
   return cudaGetLastError();
 }
 template <typename T>
