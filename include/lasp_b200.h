@@ -402,10 +402,11 @@ typedef struct {
   void* ddt_bias;
   void* kept;
   size_t kept_bytes;
-  void* ws;              /* backward: lasp_b200_scan_workspace_bytes() */
+  void* ws;              /* forward: lasp_b200_scan_forward_workspace_bytes(), which may be 0; backward: lasp_b200_scan_workspace_bytes() */
   size_t ws_bytes;
 } lasp_scan_args;
 LASP_B200_API size_t lasp_b200_scan_kept_bytes(const lasp_scan_args* a);
+LASP_B200_API size_t lasp_b200_scan_forward_workspace_bytes(const lasp_scan_args* a);
 LASP_B200_API size_t lasp_b200_scan_workspace_bytes(const lasp_scan_args* a);
 LASP_B200_API int lasp_b200_scan_forward(const lasp_scan_args* a, void* stream);
 LASP_B200_API int lasp_b200_scan_backward(const lasp_scan_args* a, void* stream);

@@ -138,6 +138,7 @@ SIGNATURES = {
     "lasp_b200_conv_backward": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
     "lasp_b200_conv_step": (C.c_int, [C.POINTER(ConvStepArgs), C.c_void_p]),
     "lasp_b200_scan_kept_bytes": (C.c_size_t, [C.POINTER(ScanArgs)]),
+    "lasp_b200_scan_forward_workspace_bytes": (C.c_size_t, [C.POINTER(ScanArgs)]),
     "lasp_b200_scan_workspace_bytes": (C.c_size_t, [C.POINTER(ScanArgs)]),
     "lasp_b200_scan_forward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),
     "lasp_b200_scan_backward": (C.c_int, [C.POINTER(ScanArgs), C.c_void_p]),

@@ -20,7 +20,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "liblasp_b200.so")
 TORCH_OPS = os.path.join(PKG, "_torch_ops.so")   # the operator as PyTorch calls it, on top of LIB
 SOURCES = ["api.cu", "split_kernels.cu", "state_kernels.cu", "fault_word.cu", "walk_kernels.cu", "wide_kernels.cu", "relay_kernels.cu", "static_scratch.cu",
-           "recurrent_api.cu", "conv_kernels.cu", "scan_forward.cu", "scan_backward.cu", "scan_step.cu"]
+           "recurrent_api.cu", "conv_kernels.cu", "scan_forward.cu", "scan_backward.cu", "scan_parts.cu", "scan_step.cu"]
 TORCH_SOURCES = ["torch_ops.cpp", "torch_recurrent.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -250,6 +250,7 @@ cudaError_t conv_step(const lasp_conv_step_args& a, cudaStream_t st);
 cudaError_t scan_forward(const lasp_scan_args& a, cudaStream_t st);
 cudaError_t scan_backward(const lasp_scan_args& a, cudaStream_t st);
 size_t scan_kept(const lasp_scan_args& a);
+size_t scan_forward_workspace(const lasp_scan_args& a);
 size_t scan_workspace(const lasp_scan_args& a);
 cudaError_t scan_step(const lasp_scan_step_args& a, cudaStream_t st);
 

@@ -63,13 +63,16 @@ int lasp_b200_conv_backward(const lasp_conv_args* a, void* stream) {
 }
 
 size_t lasp_b200_scan_kept_bytes(const lasp_scan_args* a) { return check_scan(a) == LASP_OK ? lasp::scan_kept(*a) : 0; }
+size_t lasp_b200_scan_forward_workspace_bytes(const lasp_scan_args* a) { return check_scan(a) == LASP_OK ? lasp::scan_forward_workspace(*a) : 0; }
 size_t lasp_b200_scan_workspace_bytes(const lasp_scan_args* a) { return check_scan(a) == LASP_OK ? lasp::scan_workspace(*a) : 0; }
 
 int lasp_b200_scan_forward(const lasp_scan_args* a, void* stream) {
   if (const int st = check_scan(a); st != LASP_OK) return st;
   if (a->tokens && missing(a->y)) return LASP_ERR_NULL;
-  if (reinterpret_cast<uintptr_t>(a->kept) & 15) return LASP_ERR_ALIGN;
-  if (a->kept && a->kept_bytes < lasp::scan_kept(*a)) return LASP_ERR_WORKSPACE;
+  const size_t need = lasp::scan_forward_workspace(*a);
+  if (need && !a->ws) return LASP_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(a->kept) | (need ? reinterpret_cast<uintptr_t>(a->ws) : 0)) & 15) return LASP_ERR_ALIGN;
+  if ((a->kept && a->kept_bytes < lasp::scan_kept(*a)) || a->ws_bytes < need) return LASP_ERR_WORKSPACE;
   return lasp::status_of(lasp::scan_forward(*a, static_cast<cudaStream_t>(stream)));
 }
 

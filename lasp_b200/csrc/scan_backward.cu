@@ -32,27 +32,33 @@ struct Shared {
 // What a backward pass writes beside its results, in the order of the workspace.
 struct Partial {
   float4* tokens;   // [tile][row * tokens + token][LPC][8]: of each four of states its 4 dB, 4 dC
-  float4* rates;    // [sequence][tile][kGroup]: dA, as the lanes hold it
-  float* skips;     // [sequence][2][channel]: dD, ddt_bias
+  float4* rates;    // [slot][tile][kGroup]: dA, as the lanes hold it
+  float* skips;     // [slot][2][channel]: dD, ddt_bias
 };
 
 // wide: the tensors of tokens can be read and written by kEach, B and C by four.
 template <typename T, int LPC>
-__global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a, int tiles, Partial out, bool wide) {
+__global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a, int tiles, Partial out, Cuts cuts, bool wide) {
   using TILE = Tile<LPC>;
   using SHARED = Shared<T, LPC>;
   constexpr int kEach = TILE::kEach, kVecs = TILE::kVecs, kStages = SHARED::kStages, kLead = kStages - 3;
   extern __shared__ __align__(16) char raw_smem[];
   auto& sm = *reinterpret_cast<SHARED*>(raw_smem);
   const int role = threadIdx.x / kGroup, me = threadIdx.x % kGroup;
-  const int tile_index = blockIdx.x % tiles, seq = blockIdx.x / tiles;
+  const int tile_index = blockIdx.x % tiles, slot = blockIdx.x / tiles;
   const TilePlace<TILE> tile(tile_index, a.channels, a.groups);
-  if (a.sequences && seq == a.sequences) {
+  if (slot == cuts.slots) {
     fill_outside<T, TILE>(a, a.du, tile), fill_outside<T, TILE>(a, a.ddt, tile), fill_outside<T, TILE>(a, a.dz, tile);
     return;
   }
-  const Stretch at = stretch_of(a, seq);
-  const int chunks = (at.tokens + kChunk - 1) / kChunk;   // number k of them is chunk chunks - 1 - k of the sequence
+  const Stretch at(a, slot, cuts.length);
+  if (at.index == at.count) {   // no segment: nothing to add to the sums
+    if (threadIdx.x < kGroup) out.rates[((int64_t)slot * tiles + tile_index) * kGroup + threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = threadIdx.x; e < 2 * TILE::kChannels; e += kThreads)
+      if (const int c = e % TILE::kChannels; c < tile.left) out.skips[((int64_t)slot * 2 + e / TILE::kChannels) * a.channels + tile.channel + c] = 0.f;
+    return;
+  }
+  const int chunks = (at.tokens + kChunk - 1) / kChunk;   // number k of them is chunk chunks - 1 - k of the segment
   const bool f32 = a.param_dtype == LASP_F32, gated = a.z.data != nullptr, whole = wide && tile.left >= TILE::kChannels;
   for (int c = threadIdx.x; c < TILE::kChannels; c += kThreads) {
     const bool there = c < tile.left;
@@ -68,9 +74,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
     take_registers<152>();
     const int lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
     const bool mine = ch < tile.left;
-    const int64_t state_row = ((int64_t)seq * a.channels + tile.channel + ch) * a.states;
+    const int64_t state_row = ((int64_t)at.seq * a.channels + tile.channel + ch) * a.states;
     const S4 A = mine ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
     S4 grad = mine && a.dstate_out ? s4(four_of(a.dstate_out + state_row, 4 * i, a.states)) : splat(0.f);   // a_(t+1) g_(t+1)
+    if (at.index < at.count - 1) grad = carry<TILE>(a, cuts, at, (at.index + 1) * kParts, (at.sequence_tokens - 1) / cuts.part + 1, true, grad, A, tiles, tile_index, me, ch);
     S4 dA = splat(0.f);
     const float4* kept = static_cast<const float4*>(a.kept) + ((at.chunk + chunks - 1) * tiles + tile_index) * kGroup + me;
     constexpr int kLeft = 8 / TILE::kGroups;   // of 8 sums over a warp's channels, how many a lane is left with
@@ -132,8 +139,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
       }
       __syncthreads();
     }
-    if (a.dstate_in && mine) store_four(a.dstate_in + state_row, 4 * i, a.states, f4(grad));
-    out.rates[((int64_t)seq * tiles + tile_index) * kGroup + me] = f4(dA);
+    if (a.dstate_in && mine && at.index == 0) store_four(a.dstate_in + state_row, 4 * i, a.states, f4(grad));
+    out.rates[((int64_t)slot * tiles + tile_index) * kGroup + me] = f4(dA);
   } else if (role == 1) {
     // while the states are at number k: prepare k + 2, send for k + kLead, add up k - 1
     give_registers<40>();
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
       const int which = e / TILE::kChannels, c = e % TILE::kChannels;
       float s = 0.f;
       for (int r = 0; r < kChunk; ++r) s += part[(which * kChunk + r) * TILE::kChannels + c];
-      if (c < tile.left) out.skips[((int64_t)seq * 2 + which) * a.channels + tile.channel + c] = s;
+      if (c < tile.left) out.skips[((int64_t)slot * 2 + which) * a.channels + tile.channel + c] = s;
     }
   }
 }
@@ -313,15 +320,15 @@ __global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const
   static_cast<T*>(to.data)[(int64_t)row * to.row_pitch + (int64_t)t * to.token_pitch + (int64_t)group * to.group_pitch + n] = from_f<T>(s);
 }
 
-// dA: over the sequences, in their order, a thread for each lane of a tile.
+// dA: over the slots, in their order, a thread for each lane of a tile.
 template <int LPC>
-__global__ void __launch_bounds__(kGroup) k_scan_sum_rates(lasp_scan_args a, const float4* part, int tiles, int sequences) {
+__global__ void __launch_bounds__(kGroup) k_scan_sum_rates(lasp_scan_args a, const float4* part, int tiles, int slots) {
   using TILE = Tile<LPC>;
   const TilePlace<TILE> tile(blockIdx.x, a.channels, a.groups);
   const int me = threadIdx.x, lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
   if (ch >= tile.left) return;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int q = 0; q < sequences; ++q) {
+  for (int q = 0; q < slots; ++q) {
     const float4 v = part[((int64_t)q * tiles + blockIdx.x) * kGroup + me];
     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
   }
@@ -330,25 +337,29 @@ __global__ void __launch_bounds__(kGroup) k_scan_sum_rates(lasp_scan_args a, con
 
 // dD, ddt_bias: the same.
 template <typename T>
-__global__ void __launch_bounds__(256) k_scan_sum_skips(lasp_scan_args a, const float* part, int sequences) {
+__global__ void __launch_bounds__(256) k_scan_sum_skips(lasp_scan_args a, const float* part, int slots) {
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
   void* to = blockIdx.y ? a.ddt_bias : a.dD;
   if (c >= a.channels || !to) return;
   float s = 0.f;
-  for (int q = 0; q < sequences; ++q) s += part[((int64_t)q * 2 + blockIdx.y) * a.channels + c];
+  for (int q = 0; q < slots; ++q) s += part[((int64_t)q * 2 + blockIdx.y) * a.channels + c];
   store_param<T>(to, a.param_dtype == LASP_F32, c, s);
 }
 
 struct Plan {
-  int tiles, sequences;
-  size_t tokens, rates, skips;   // floats
+  int tiles;
+  Cuts cuts;
+  size_t tokens, rates, skips, parts;   // floats
 };
 template <int LPC>
 Plan plan_as(const lasp_scan_args& a) {
+  using TILE = Tile<LPC>;
   Plan p;
-  p.tiles = tiles_of<Tile<LPC>>(a.channels, a.groups), p.sequences = a.sequences ? a.sequences : a.rows;
+  p.tiles = tiles_of<TILE>(a.channels, a.groups);
+  const Cuts cuts = cuts_of<TILE>(a, p.tiles, true, nullptr);
   p.tokens = (size_t)p.tiles * a.rows * a.tokens * 8 * LPC;
-  p.rates = (size_t)p.sequences * p.tiles * kGroup * 4, p.skips = (size_t)p.sequences * 2 * a.channels;
+  p.rates = (size_t)cuts.slots * p.tiles * kGroup * 4, p.skips = ((size_t)cuts.slots * 2 * a.channels + 3) / 4 * 4, p.parts = (size_t)floats_of<TILE>(cuts, p.tiles);
+  p.cuts = cuts_of<TILE>(a, p.tiles, true, static_cast<float*>(a.ws) + p.tokens + p.rates + p.skips);
   return p;
 }
 
@@ -364,12 +375,14 @@ cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
   const Partial out{reinterpret_cast<float4*>(ws), reinterpret_cast<float4*>(ws + p.tokens), ws + p.tokens + p.rates};
   bool wide = (a.channels / a.groups) % TILE::kEach == 0 && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
   for (const lasp_tokens* t : {&a.u, &a.dt, &a.z, &a.dy, &a.du, &a.ddt, &a.dz}) wide = wide && reads_by<T>(*t, TILE::kEach);
-  kernel<<<(unsigned)(p.tiles * (p.sequences + (a.sequences ? 1 : 0))), kThreads, smem, st>>>(a, p.tiles, out, wide);
+  if (p.cuts.length != kUncut)
+    if (const cudaError_t e = scan_parts<T, LPC>(a, p.cuts, p.tiles, true, st); e != cudaSuccess) return e;
+  kernel<<<(unsigned)(p.tiles * (p.cuts.slots + (a.sequences ? 1 : 0))), kThreads, smem, st>>>(a, p.tiles, out, p.cuts, wide);
   const int64_t per_group = (int64_t)a.rows * a.tokens * 8 * LPC;
   if (per_group)
     k_scan_sum_tokens<T><<<dim3((unsigned)((per_group + 255) / 256), a.groups), 256, 0, st>>>(a, reinterpret_cast<const float*>(out.tokens), p.tiles, LPC);
-  if (a.dA) k_scan_sum_rates<LPC><<<p.tiles, kGroup, 0, st>>>(a, out.rates, p.tiles, p.sequences);
-  if (a.dD || a.ddt_bias) k_scan_sum_skips<T><<<dim3((a.channels + 255) / 256, 2), 256, 0, st>>>(a, out.skips, p.sequences);
+  if (a.dA) k_scan_sum_rates<LPC><<<p.tiles, kGroup, 0, st>>>(a, out.rates, p.tiles, (int)p.cuts.slots);
+  if (a.dD || a.ddt_bias) k_scan_sum_skips<T><<<dim3((a.channels + 255) / 256, 2), 256, 0, st>>>(a, out.skips, (int)p.cuts.slots);
   return cudaGetLastError();
 }
 
@@ -395,7 +408,7 @@ cudaError_t scan_backward(const lasp_scan_args& a, cudaStream_t st) {
 size_t scan_kept(const lasp_scan_args& a) { return (size_t)chunks_of(a) * plan_of(a).tiles * kGroup * sizeof(float4); }
 size_t scan_workspace(const lasp_scan_args& a) {
   const Plan p = plan_of(a);
-  return (p.tokens + p.rates + p.skips) * sizeof(float);
+  return (p.tokens + p.rates + p.skips + p.parts) * sizeof(float);
 }
 
 }  // namespace lasp

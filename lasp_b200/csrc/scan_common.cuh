@@ -200,22 +200,85 @@ int tiles_of(int channels, int groups) {
   return groups * ((in_group + TILE::kChannels - 1) / TILE::kChannels);
 }
 
-// Where a sequence's tokens lie: row and first token, and the number of its first chunk among all chunks, as the kept states are
-// counted.  A row of n tokens has ceil(n / kChunk) of them; packed sequence i those from offsets[i] / kChunk + i on, which leaves
-// room for each.
-struct Stretch {
-  int row, begin, tokens;
-  int64_t chunk;
+// Few channels and sequences leave SMs idle.  Their tokens are then cut into segments of `length`, one for a block; where a segment starts
+// (forward: the state, backward: the gradient that comes in from behind) is put together from what the parts of the others, kParts to a
+// segment, do to a state of zero (`ends`) and from the sums of their steps, whose exponentials are the parts' decays: a first pass over
+// the tokens (scan_parts.cu) finds those.  It takes the exponentials once more, so segments come only where they are that many.
+constexpr int kParts = 4, kUncut = 0x7ffffff0;
+// Tokens of a segment; segments for which the first pass pays, forward and backward.  us without and with, bf16, 16 states: 4096 tokens of
+// 1024 channels 157 and 69, 602 and 169; 16384 of 4096 (two segments) 612 and 933, 2418 and 2085; three forward 613 and 653.
+constexpr int kLeast = 128, kLeastForward = 4, kLeastBack = 2;
+struct Cuts {
+  int length, part;       // tokens of a segment, of a part: multiples of kChunk, or kUncut
+  int64_t slots, parts;   // how many there may be
+  float4* ends;           // [part][tile][kGroup]: four states of each lane
+  float* steps;           // [part][tile][channel of the tile]
 };
-__device__ __forceinline__ Stretch stretch_of(const lasp_scan_args& a, int seq) {
-  if (!a.sequences) return {seq, 0, a.tokens, (int64_t)seq * ((a.tokens + kChunk - 1) / kChunk)};
-  int begin, end;
-  Sequences{a.offsets, a.index_bits, a.sequences, a.tokens}.bounds(seq, &begin, &end);
-  return {0, begin, end - begin, (int64_t)begin / kChunk + seq};
+
+// Slots: a row of n tokens has ceil(n / length) of them, one at least; packed sequence i those from offsets[i] / length + i on, which
+// leaves room for each.  Chunks, as the kept states are counted, are slots of kChunk.
+__device__ __forceinline__ int64_t slot_of(const lasp_scan_args& a, int seq, int begin, int length) {
+  return a.sequences ? (int64_t)(begin / length) + seq : (int64_t)seq * (a.tokens > 0 ? (a.tokens - 1) / length + 1 : 1);
 }
-inline int64_t chunks_of(const lasp_scan_args& a) {
-  return a.sequences ? (int64_t)a.tokens / kChunk + a.sequences + 1 : (int64_t)a.rows * ((a.tokens + kChunk - 1) / kChunk);
+inline int64_t slots_of(const lasp_scan_args& a, int length) {
+  return a.sequences ? (int64_t)a.tokens / length + a.sequences : (int64_t)a.rows * (a.tokens > 0 ? (a.tokens - 1) / length + 1 : 1);
 }
+inline int64_t chunks_of(const lasp_scan_args& a) { return slots_of(a, kChunk); }
+
+// What a slot holds: segment `index` of the `count` of a sequence (none: index = count), the row, the first and the number of its tokens and
+// of the sequence's, and the number of its first chunk.
+struct Stretch {
+  int seq, index, count, row, begin, tokens, sequence_begin, sequence_tokens;
+  int64_t chunk;
+  __device__ __forceinline__ Stretch(const lasp_scan_args& a, int slot, int length) {
+    int& all = sequence_tokens;
+    all = a.tokens, sequence_begin = 0;
+    if (!a.sequences) {
+      count = a.tokens > 0 ? (a.tokens - 1) / length + 1 : 1;
+      seq = row = slot / count;
+    } else {
+      const Sequences s{a.offsets, a.index_bits, a.sequences, a.tokens};
+      int lo = 0, hi = a.sequences;   // (the slots of sequences [0, lo) begin at or before this one)
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s.at(mid) / length + mid <= slot)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      seq = max(lo - 1, 0), row = 0;
+      int end;
+      s.bounds(seq, &sequence_begin, &end);
+      all = end - sequence_begin;
+      count = all > 0 ? (all - 1) / length + 1 : 1;
+    }
+    const int i = a.sequences ? slot - sequence_begin / length - seq : slot - seq * count;
+    index = i < 0 || i >= count ? count : i;
+    const int first = index < count ? index * length : 0;
+    begin = sequence_begin + first, tokens = index < count ? min(length, all - first) : 0;
+    chunk = slot_of(a, seq, sequence_begin, kChunk) + first / kChunk;
+  }
+};
+
+// Four of a lane's states (`me` of the tile's lanes, channel ch) taken from one end of parts [lo, hi) of a sequence to the other: forwards, or back.
+template <class TILE>
+__device__ __forceinline__ S4 carry(const lasp_scan_args& a, const Cuts& cuts, const Stretch& at, int lo, int hi, bool back, S4 from, S4 A, int tiles, int tile, int me, int ch) {
+  const int64_t first = slot_of(a, at.seq, at.sequence_begin, cuts.part);
+#pragma unroll 4
+  for (int p = lo; p < hi; ++p) {
+    const int64_t k = (first + (back ? lo + hi - 1 - p : p)) * tiles + tile;
+    const float half = 0.5f * cuts.steps[k * TILE::kChannels + ch];
+    float d[4];   // the decay's root, taken twice: what is zero stays so where the decay itself is beyond fp32
+    const float4 x = f4(exp2(mul(A, f2(half, half))));
+    d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) d[n] = d[n] > 3.402823466e38f ? 3.402823466e38f : d[n];
+    const S4 root = s4(make_float4(d[0], d[1], d[2], d[3]));
+    from = fma(root, mul(root, from), s4(cuts.ends[k * kGroup + me]));
+  }
+  return from;
+}
+
 // n neighbouring numbers of a tensor of tokens can be read and written by accesses of all their bytes, or of 16.
 template <typename T>
 bool reads_by(const lasp_tokens& t, int n) { return by(t, std::min<size_t>(16, n * sizeof(T)), sizeof(T)); }
@@ -244,5 +307,25 @@ __device__ void fill_outside(const lasp_scan_args& a, const lasp_tokens& y, cons
     if (c < tile.left) p[(int64_t)t * y.token_pitch + c] = from_f<T>(0.f);
   }
 }
+
+// Floats that the parts' ends and steps take.
+template <class TILE>
+int64_t floats_of(const Cuts& c, int tiles) { return c.length == kUncut ? 0 : c.parts * tiles * (4 * kGroup + TILE::kChannels); }
+template <class TILE>
+Cuts cuts_of(const lasp_scan_args& a, int tiles, bool backward, float* ws) {
+  Cuts c{kUncut, kUncut, 0, 0, nullptr, nullptr};
+  // two blocks an SM, no more (sequences of a packed row: as many tokens for each as if there were one)
+  const int64_t unit = kParts * kChunk, segments = 2 * std::max(1, sm_count()) / ((int64_t)tiles * a.rows);
+  if (segments >= 2) {
+    const int64_t length = std::max<int64_t>(kLeast, ((a.tokens + segments - 1) / segments + unit - 1) / unit * unit);
+    if (a.tokens > (backward ? kLeastBack - 1 : kLeastForward - 1) * length) c.length = (int)length, c.part = c.length / kParts;
+  }
+  c.slots = slots_of(a, c.length), c.parts = slots_of(a, c.part);
+  c.ends = reinterpret_cast<float4*>(ws), c.steps = ws + c.parts * tiles * 4 * kGroup;
+  return c;
+}
+// The first pass: ends and steps of the parts that a segment needs.
+template <typename T, int LPC>
+cudaError_t scan_parts(const lasp_scan_args& a, const Cuts& cuts, int tiles, bool backward, cudaStream_t st);
 
 }  // namespace lasp

@@ -21,16 +21,17 @@ struct Shared {
 
 // wide: u, dt, z, y can be read and written by kEach, B and C by four.
 template <typename T, int LPC>
-__global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, int tiles, bool wide) {
+__global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, int tiles, Cuts cuts, bool wide) {
   using TILE = Tile<LPC>;
   constexpr int kEach = TILE::kEach, kVecs = TILE::kVecs;
   extern __shared__ __align__(16) char raw_smem[];
   auto& sm = *reinterpret_cast<Shared<T, LPC>*>(raw_smem);
   const int role = threadIdx.x / kGroup, me = threadIdx.x % kGroup;
-  const int tile_index = blockIdx.x % tiles, seq = blockIdx.x / tiles;
+  const int tile_index = blockIdx.x % tiles, slot = blockIdx.x / tiles;
   const TilePlace<TILE> tile(tile_index, a.channels, a.groups);
-  if (a.sequences && seq == a.sequences) return fill_outside<T, TILE>(a, a.y, tile);
-  const Stretch at = stretch_of(a, seq);
+  if (slot == cuts.slots) return fill_outside<T, TILE>(a, a.y, tile);
+  const Stretch at(a, slot, cuts.length);
+  if (at.index == at.count) return;
   const int chunks = (at.tokens + kChunk - 1) / kChunk;
   const bool f32 = a.param_dtype == LASP_F32, gated = a.z.data != nullptr, whole = wide && tile.left >= TILE::kChannels;
   for (int c = threadIdx.x; c < TILE::kChannels; c += kThreads) {
@@ -47,9 +48,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
     take_registers<144>();
     const int lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
     const bool mine = ch < tile.left;
-    const int64_t state_row = ((int64_t)seq * a.channels + tile.channel + ch) * a.states;
+    const int64_t state_row = ((int64_t)at.seq * a.channels + tile.channel + ch) * a.states;
     const S4 A = mine ? rates(a.A + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states) : splat(0.f);
     S4 h = mine && a.state_in ? s4(four_of(a.state_in + state_row, 4 * i, a.states)) : splat(0.f);
+    if (at.index) h = carry<TILE>(a, cuts, at, 0, at.index * kParts, false, h, A, tiles, tile_index, me, ch);
     float4* kept = a.kept ? static_cast<float4*>(a.kept) + (at.chunk * tiles + tile_index) * kGroup + me : nullptr;
     constexpr int kTurn = 8, kRound = LPC < kTurn ? LPC : kTurn, kSame = LPC / kRound;   // tokens taken, and summed, at a time
     S4 decay[kTurn], state[kTurn];   // state: first what a token puts in, then the state behind it
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
       buf = next;
       __syncthreads();
     }
-    if (a.state_out && mine) store_four(a.state_out + state_row, 4 * i, a.states, f4(h));
+    if (a.state_out && mine && at.index == at.count - 1) store_four(a.state_out + state_row, 4 * i, a.states, f4(h));
   } else if (role == 1) {
     give_registers<48>();
     static_assert(TILE::kUnits <= kGroup, "a thread has at most one unit of each tensor");
@@ -188,10 +190,13 @@ cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
   const cudaError_t err = ready<kernel>(smem);
   if (err != cudaSuccess) return err;
   const int tiles = tiles_of<TILE>(a.channels, a.groups);
-  const int sequences = a.sequences ? a.sequences + 1 : a.rows;   // (one more: what lies in none)
+  const Cuts cuts = cuts_of<TILE>(a, tiles, false, static_cast<float*>(a.ws));
   const bool wide = (a.channels / a.groups) % TILE::kEach == 0 && reads_by<T>(a.u, TILE::kEach) && reads_by<T>(a.dt, TILE::kEach) &&
                     reads_by<T>(a.z, TILE::kEach) && reads_by<T>(a.y, TILE::kEach) && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
-  kernel<<<(unsigned)(tiles * sequences), kThreads, smem, st>>>(a, tiles, wide);
+  if (cuts.length != kUncut)
+    if (const cudaError_t e = scan_parts<T, LPC>(a, cuts, tiles, false, st); e != cudaSuccess) return e;
+  // (one slot more: what lies in no sequence)
+  kernel<<<(unsigned)(tiles * (cuts.slots + (a.sequences ? 1 : 0))), kThreads, smem, st>>>(a, tiles, cuts, wide);
   return cudaGetLastError();
 }
 
@@ -204,8 +209,18 @@ cudaError_t forward_as(const lasp_scan_args& a, cudaStream_t st) {
   }
 }
 
+template <int LPC>
+size_t workspace_as(const lasp_scan_args& a) {
+  const int tiles = tiles_of<Tile<LPC>>(a.channels, a.groups);
+  return (size_t)floats_of<Tile<LPC>>(cuts_of<Tile<LPC>>(a, tiles, false, nullptr), tiles) * sizeof(float);
+}
+
 }  // namespace
 
+size_t scan_forward_workspace(const lasp_scan_args& a) {
+  const int padded = padded_states(a.states);
+  return padded == 16 ? workspace_as<4>(a) : padded == 32 ? workspace_as<8>(a) : workspace_as<16>(a);
+}
 cudaError_t scan_forward(const lasp_scan_args& a, cudaStream_t st) {
   return a.dtype == LASP_F32 ? forward_as<float>(a, st) : a.dtype == LASP_BF16 ? forward_as<__nv_bfloat16>(a, st) : forward_as<__half>(a, st);
 }

@@ -279,6 +279,11 @@ variable_list run_scan(const ScanInputs& s, bool want_state, bool keep) {   // y
     kept = at::empty({(int64_t)lasp_b200_scan_kept_bytes(&a)}, s.u.options().dtype(at::kByte));
     a.kept = kept.data_ptr(), a.kept_bytes = (size_t)kept.numel();
   }
+  Tensor ws;
+  if (const size_t need = lasp_b200_scan_forward_workspace_bytes(&a)) {
+    ws = at::empty({(int64_t)need}, s.u.options().dtype(at::kByte));
+    a.ws = ws.data_ptr(), a.ws_bytes = need;
+  }
   Range range("lasp_b200_scan_forward");
   check_status("lasp_b200_scan_forward", lasp_b200_scan_forward(&a, at::cuda::getCurrentCUDAStream().stream()));
   return {y, last, kept};

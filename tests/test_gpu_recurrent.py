@@ -122,6 +122,33 @@ def test_scan(b, n, c, N, groups, cu, dtype, ptype, gate, softplus, strided, ful
     assert torch.equal(alone, y)
 
 
+SEGMENTS = [   # few channels and many tokens: sequences are cut into segments (of 256 tokens and more), some of whose lengths are odd
+    (1, 1301, 20, 16, 1, None, F32, F32, True, True, True),
+    (2, 1025, 40, 32, 1, None, BF16, F32, True, True, False),
+    (1, 777, 9, 64, 1, None, F16, F32, False, True, True),
+    (1, 2113, 36, 16, 2, [3, 3, 903, 904, 1416, 2100], F32, F32, True, True, True),
+    (1, 2049, 16, 24, 1, [0, 1, 258, 2049, 2049], BF16, F32, True, False, False),
+]
+
+
+@pytest.mark.parametrize("b,n,c,N,groups,cu,dtype,ptype,gate,softplus,strided", SEGMENTS)
+@pytest.mark.parametrize("full", [True, False])
+def test_scan_in_segments(b, n, c, N, groups, cu, dtype, ptype, gate, softplus, strided, full):
+    test_scan(b, n, c, N, groups, cu, dtype, ptype, gate, softplus, strided, full)
+
+
+def test_a_state_of_zero_stays_so_where_rates_grow():
+    """A above zero: the decay of a whole segment is beyond fp32, that of a token is not."""
+    from lasp_b200 import selective_scan
+    n, c, N = 1400, 8, 16
+    u, dt = torch.zeros(1, n, c, device=DEV), torch.ones(1, n, c, device=DEV)
+    B, C = torch.ones(1, n, N, device=DEV), torch.ones(1, n, N, device=DEV)
+    leaf = u.requires_grad_(True)
+    y, last = selective_scan(leaf, dt, torch.full((c, N), 0.5, device=DEV), B, C, return_state=True)
+    assert not y.any() and not last.any()
+    assert not torch.autograd.grad(y, leaf, torch.zeros_like(y))[0].any()
+
+
 # ---- single tokens -------------------------------------------------------------------------------------------------------------------
 STEP = [
     # rows, slots, channels, states, groups, dtype, parameters' type, gate, softplus
