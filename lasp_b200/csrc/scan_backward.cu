@@ -21,8 +21,8 @@ struct Shared {
   static constexpr int kStages = sizeof(T) == 4 ? 6 : 7;   // chunks that are here, or on their way, as they are in global memory
   Vec<T, TILE::kEach> u[kStages][TILE::kUnits], dt[kStages][TILE::kUnits], z[kStages][TILE::kUnits], dy[kStages][TILE::kUnits];
   Vec<T, 4> B[kStages][TILE::kStateUnits], C[kStages][TILE::kStateUnits];
-  float4 step[3][kChunk][TILE::kChannels];          // dt, dt, dt u, dt u: in pairs, as packed operations take them
-  float2 d[3][kChunk][TILE::kChannels];             // d, d
+  float2 step[3][kChunk][TILE::kChannels];          // dt, dt u
+  float d[3][kChunk][TILE::kChannels];
   float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
   float y[2][kChunk][TILE::kChannels + 4], gB[2][kChunk][TILE::kChannels + 4], eA[2][kChunk][TILE::kChannels + 4];   // <C, h>, <g, B>, <e, A>
   float4 sums[2][kChunk][4][kSumsOfToken * LPC / 4];   // of each warp
@@ -91,37 +91,39 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
       kept -= (int64_t)tiles * kGroup;
       if (k + 1 < chunks) first = *kept;
       S4 decay[kHalf], h[kHalf];
-      const auto decays = [&](int t0) {
+      const auto ahead = [&](int t0) {   // decays, and in h what the tokens put in
 #pragma unroll
-        for (int t = 0; t < kHalf; ++t) decay[t] = exp2(mul(A, pair_of(&sm.step[buf][t0 + t][ch])));
-      };
-      const auto up = [&](int t0, int t, S4 before) {
-        return fma(decay[t], before, mul(load4(&sm.B4[buf][t0 + t][i]), pair_of(reinterpret_cast<const float2*>(&sm.step[buf][t0 + t][ch]) + 1)));
+        for (int t = 0; t < kHalf; ++t) {
+          const float2 step = sm.step[buf][t0 + t][ch];
+          decay[t] = exp2(mul(A, f2(step.x, step.x)));
+          h[t] = mul(load4(&sm.B4[buf][t0 + t][i]), f2(step.y, step.y));
+        }
       };
       S4 middle = start;
-      decays(0);
+      ahead(0);
 #pragma unroll
-      for (int t = 0; t < kHalf; ++t) middle = up(0, t, middle);
+      for (int t = 0; t < kHalf; ++t) middle = fma(decay[t], middle, h[t]);
 #pragma unroll
       for (int half = 1; half >= 0; --half) {
         const S4 before = half ? middle : start;
-        decays(half * kHalf);
+        ahead(half * kHalf);
 #pragma unroll
-        for (int t = 0; t < kHalf; ++t) h[t] = up(half * kHalf, t, t ? h[t - 1] : before);
+        for (int t = 0; t < kHalf; ++t) h[t] = fma(decay[t], t ? h[t - 1] : before, h[t]);
 #pragma unroll
         for (int r = kHalf - kRound; r >= 0; r -= kRound) {
           float y[kRound], gB[kRound], eA[kRound], over[kRound][kLeft];   // (all stored together: what lies in between could not be read ahead)
 #pragma unroll
           for (int q = kRound - 1; q >= 0; --q) {
             const int t = half * kHalf + r + q;
-            const S4 step = load4(&sm.step[buf][t][ch]), B = load4(&sm.B4[buf][t][i]), C = load4(&sm.C4[buf][t][i]), &now = h[r + q];
-            const F2 d = pair_of(&sm.d[buf][t][ch]);
-            const S4 g = fma(C, d, grad), dB = mul(g, step.b), dC = mul(now, d);
+            const float2 step = sm.step[buf][t][ch];
+            const S4 B = load4(&sm.B4[buf][t][i]), C = load4(&sm.C4[buf][t][i]), &now = h[r + q];
+            const F2 d = f2(sm.d[buf][t][ch], sm.d[buf][t][ch]);
+            const S4 g = fma(C, d, grad), dB = mul(g, f2(step.y, step.y)), dC = mul(now, d);
             y[q] = dot(C, now), gB[q] = dot(B, g);
             grad = mul(decay[r + q], g);
             const S4 e = mul(grad, r + q ? h[r + q - 1] : before);
             eA[q] = dot(e, A);
-            dA = fma(e, step.a, dA);
+            dA = fma(e, f2(step.x, step.x), dA);
             float v[8];
             apart(dB.a, v[0], v[1]), apart(dB.b, v[2], v[3]), apart(dC.a, v[4], v[5]), apart(dC.b, v[6], v[7]);
             sum_over<8, TILE::kGroups, 1>(v, lane);
@@ -211,9 +213,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
             if (a.softplus) s = softplus(s);
             float x, y, ix, iy;
             apart(s, x, y), apart(mul2(s, f2(u[q], u[q + 1])), ix, iy);
-            sm.step[buf][row][c0 + q] = there ? make_float4(x, x, ix, ix) : make_float4(0.f, 0.f, 0.f, 0.f);
-            sm.step[buf][row][c0 + q + 1] = there ? make_float4(y, y, iy, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(&sm.d[buf][row][c0 + q]) = there ? make_float4(d[q], d[q], d[q + 1], d[q + 1]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + q]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float2*>(&sm.d[buf][row][c0 + q]) = there ? make_float2(d[q], d[q + 1]) : make_float2(0.f, 0.f);
           }
         }
 #pragma unroll
