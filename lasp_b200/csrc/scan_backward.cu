@@ -8,7 +8,7 @@
 // chunk up from the state that the forward pass has kept ahead of it, and then half a chunk at a time: up for the states, down for the
 // gradients, with the decays and states of eight tokens in registers.  (Those of 16 do not fit, and a state kept for every eighth
 // token would cost 32 bytes of memory for every eight tokens and state more than the 8 exponentials that the first half takes twice.)  dB and dC are sums over channels: each block leaves
-// its tile's, and k_scan_sum_tokens adds those up in the order of the tiles, so that results do not depend on when blocks run.
+// its tile's, and k_scan_sums adds those up in the order of the tiles, so that results do not depend on when blocks run.
 #include "scan_common.cuh"
 
 namespace lasp {
@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
 #pragma unroll
         for (int t = 0; t < kHalf; ++t) {
           const float2 step = sm.step[buf][t0 + t][ch];
-          decay[t] = exp2(mul(A, f2(step.x, step.x)));
+          decay[t] = decay_of(A, step.x);
           h[t] = mul(load4(&sm.B4[buf][t0 + t][i]), f2(step.y, step.y));
         }
       };
-      S4 middle = start;
+      S4 middle = start, e_sum = splat(0.f);   // (dA of the chunk: added up by themselves, sums of many tokens lose half as many bits)
       ahead(0);
 #pragma unroll
       for (int t = 0; t < kHalf; ++t) middle = fma(decay[t], middle, h[t]);
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
             grad = mul(decay[r + q], g);
             const S4 e = mul(grad, r + q ? h[r + q - 1] : before);
             eA[q] = dot(e, A);
-            dA = fma(e, f2(step.x, step.x), dA);
+            e_sum = fma(e, f2(step.x, step.x), e_sum);
             float v[8];
             apart(dB.a, v[0], v[1]), apart(dB.b, v[2], v[3]), apart(dC.a, v[4], v[5]), apart(dC.b, v[6], v[7]);
             sum_over<8, TILE::kGroups, 1>(v, lane);
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
           }
         }
       }
+      dA = {add2(dA.a, e_sum.a), add2(dA.b, e_sum.b)};
       __syncthreads();
     }
     if (a.dstate_in && mine && at.index == 0) store_four(a.dstate_in + state_row, 4 * i, a.states, f4(grad));
@@ -297,53 +298,62 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
   }
 }
 
-// dB, dC of a token: over the tiles of its group, in their order.
-template <typename T>
-__global__ void __launch_bounds__(256) k_scan_sum_tokens(lasp_scan_args a, const float* part, int tiles, int lpc) {
-  const int64_t all = (int64_t)a.rows * a.tokens, wide = 8 * lpc, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= all * wide) return;
-  const int group = blockIdx.y, in_group = tiles / a.groups;
-  const int64_t token = e / wide;
-  const int at = (int)(e % wide), number = at % 8, n = at / 8 * 4 + number % 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
-  if (n >= a.states) return;
-  float s = 0.f;
-  bool inside = true;
-  if (a.sequences) {
-    const Sequences q{a.offsets, a.index_bits, a.sequences, a.tokens};
-    inside = t >= q.at(0) && t < q.at(a.sequences);
-  }
-  if (inside) {
-    const float* p = part + (int64_t)group * in_group * all * wide + e;
-#pragma unroll 8
-    for (int k = 0; k < in_group; ++k) s += p[(int64_t)k * all * wide];
-  }
-  const lasp_tokens& to = number < 4 ? a.dB : a.dC;
-  static_cast<T*>(to.data)[(int64_t)row * to.row_pitch + (int64_t)t * to.token_pitch + (int64_t)group * to.group_pitch + n] = from_f<T>(s);
-}
-
-// dA: over the slots, in their order, a thread for each lane of a tile.
-template <int LPC>
-__global__ void __launch_bounds__(kGroup) k_scan_sum_rates(lasp_scan_args a, const float4* part, int tiles, int slots) {
+// What the blocks have left is added up by one launch whose blocks are of three kinds, each in a fixed order: dB and dC over the tiles of a
+// group (a block takes kSumFours fours of numbers and kSumRanges ranges of tiles at once), then dA, then dD and ddt_bias over the slots.
+constexpr int kSumThreads = 256, kSumRanges = 8, kSumFours = kSumThreads / kSumRanges;
+template <typename T, int LPC>
+__global__ void __launch_bounds__(kSumThreads) k_scan_sums(lasp_scan_args a, Partial part, int tiles, int slots, int64_t token_blocks) {
   using TILE = Tile<LPC>;
-  const TilePlace<TILE> tile(blockIdx.x, a.channels, a.groups);
-  const int me = threadIdx.x, lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
-  if (ch >= tile.left) return;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int q = 0; q < slots; ++q) {
-    const float4 v = part[((int64_t)q * tiles + blockIdx.x) * kGroup + me];
-    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  const int me = threadIdx.x;
+  int64_t block = blockIdx.x;
+  const auto add = [](float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
+  if (block < token_blocks * a.groups) {
+    __shared__ float4 ranges[kSumRanges][kSumFours];
+    constexpr int kFours = kSumsOfToken * LPC / 4;   // of a token
+    const int group = (int)(block / token_blocks), in_group = tiles / a.groups, range = me / kSumFours;
+    const int64_t all = (int64_t)a.rows * a.tokens * kFours, e = (block - group * token_blocks) * kSumFours + me % kSumFours, token = e / kFours;
+    const int at = (int)(e % kFours), n = at / 2 * 4, row = (int)(token / a.tokens), t = (int)(token - (int64_t)row * a.tokens);
+    bool inside = e < all;
+    if (a.sequences) {
+      const Sequences q{a.offsets, a.index_bits, a.sequences, a.tokens};
+      inside = inside && t >= q.at(0) && t < q.at(a.sequences);
+    }
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (inside) {
+      const float4* p = part.tokens + (int64_t)group * in_group * all + e;
+      const int each = (in_group + kSumRanges - 1) / kSumRanges, end = min(in_group, (range + 1) * each);
+#pragma unroll 8
+      for (int k = range * each; k < end; ++k) add(s, p[k * all]);
+    }
+    ranges[range][me % kSumFours] = s;
+    __syncthreads();
+    if (range || e >= all) return;
+#pragma unroll
+    for (int r = 1; r < kSumRanges; ++r) add(s, ranges[r][me]);
+    const lasp_tokens& to = at % 2 ? a.dC : a.dB;
+    T* out = static_cast<T*>(to.data) + (int64_t)row * to.row_pitch + (int64_t)t * to.token_pitch + (int64_t)group * to.group_pitch + n;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < a.states) out[k] = from_f<T>(v[k]);
+    return;
   }
-  store_four(a.dA + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states, s);
-}
-
-// dD, ddt_bias: the same.
-template <typename T>
-__global__ void __launch_bounds__(256) k_scan_sum_skips(lasp_scan_args a, const float* part, int slots) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  void* to = blockIdx.y ? a.ddt_bias : a.dD;
+  block -= token_blocks * a.groups;
+  if (block < tiles) {   // dA: a thread for each lane of a tile
+    const TilePlace<TILE> tile((int)block, a.channels, a.groups);
+    const int lane = me % 32, i = lane / TILE::kGroups, ch = me / 32 * TILE::kGroups + lane % TILE::kGroups;
+    if (!a.dA || me >= kGroup || ch >= tile.left) return;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < slots; ++q) add(s, part.rates[((int64_t)q * tiles + block) * kGroup + me]);
+    store_four(a.dA + (int64_t)(tile.channel + ch) * a.states, 4 * i, a.states, s);
+    return;
+  }
+  const int64_t c = (block - tiles) / 2 * kSumThreads + me;
+  const int which = (int)((block - tiles) % 2);
+  void* to = which ? a.ddt_bias : a.dD;
   if (c >= a.channels || !to) return;
   float s = 0.f;
-  for (int q = 0; q < slots; ++q) s += part[((int64_t)q * 2 + blockIdx.y) * a.channels + c];
+  for (int q = 0; q < slots; ++q) s += part.skips[((int64_t)q * 2 + which) * a.channels + c];
   store_param<T>(to, a.param_dtype == LASP_F32, c, s);
 }
 
@@ -379,11 +389,9 @@ cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
   if (p.cuts.length != kUncut)
     if (const cudaError_t e = scan_parts<T, LPC>(a, p.cuts, p.tiles, true, st); e != cudaSuccess) return e;
   kernel<<<(unsigned)(p.tiles * (p.cuts.slots + (a.sequences ? 1 : 0))), kThreads, smem, st>>>(a, p.tiles, out, p.cuts, wide);
-  const int64_t per_group = (int64_t)a.rows * a.tokens * 8 * LPC;
-  if (per_group)
-    k_scan_sum_tokens<T><<<dim3((unsigned)((per_group + 255) / 256), a.groups), 256, 0, st>>>(a, reinterpret_cast<const float*>(out.tokens), p.tiles, LPC);
-  if (a.dA) k_scan_sum_rates<LPC><<<p.tiles, kGroup, 0, st>>>(a, out.rates, p.tiles, (int)p.cuts.slots);
-  if (a.dD || a.ddt_bias) k_scan_sum_skips<T><<<dim3((a.channels + 255) / 256, 2), 256, 0, st>>>(a, out.skips, (int)p.cuts.slots);
+  const int64_t token_blocks = ((int64_t)a.rows * a.tokens * (kSumsOfToken * LPC / 4) + kSumFours - 1) / kSumFours;
+  const int64_t blocks = token_blocks * a.groups + p.tiles + 2 * (((int64_t)a.channels + kSumThreads - 1) / kSumThreads);
+  k_scan_sums<T, LPC><<<(unsigned)blocks, kSumThreads, 0, st>>>(a, out, p.tiles, (int)p.cuts.slots, token_blocks);
   return cudaGetLastError();
 }
 

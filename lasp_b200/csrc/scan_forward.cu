@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
     S4 decay[kTurn], state[kTurn];   // state: first what a token puts in, then the state behind it
     const auto ahead = [&](int buf, int t0, int t) {   // of token t0 + t
       const float2 step = sm.step[buf][t0 + t][ch];
-      decay[t] = exp2(mul(A, f2(step.x, step.x)));
+      decay[t] = decay_of(A, step.x);
       state[t] = mul(load4(&sm.B4[buf][t0 + t][i]), f2(step.y, step.y));
     };
     __syncthreads();   // chunk 0 is here

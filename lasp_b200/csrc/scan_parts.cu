@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kGroup, 5) k_scan_parts(lasp_scan_args a, int 
     for (int s = 0; s < kTake; ++s) {
       const int t = BACK ? kTake - 1 - s : s;
       const float2 x = step[buf][t][ch];
-      const S4 decay = exp2(mul(A, f2(x.x, x.x))), v = load4(&four[buf][t][i]);
+      const S4 decay = decay_of(A, x.x), v = load4(&four[buf][t][i]);
       sum += x.x;
       h = BACK ? mul(decay, fma(v, f2(x.y, x.y), h)) : fma(decay, h, mul(v, f2(x.y, x.y)));
     }

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepBlocks) k_scan_step(lasp_sc
         if constexpr (!WHOLE)
           if (const int64_t g = (c0 + k) / in_group; k && k < own && (c0 + k) % in_group == 0)
             B = s4_of(four(at(pB + g * a.B.group_pitch, a.B.row_pitch, r))), C = s4_of(four(at(pC + g * a.C.group_pitch, a.C.row_pitch, r)));
-        h[k] = fma(exp2(mul(rate[k], f2(dt, dt))), h[k], mul(B, f2(x, x)));
+        h[k] = fma(decay_of(rate[k], dt), h[k], mul(B, f2(x, x)));
         y[k] = dot(h[k], C);
       }
       sum_over<kOwn, LPC, 1>(y, lane);
