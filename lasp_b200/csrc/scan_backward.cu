@@ -24,9 +24,9 @@ struct Shared {
   float2 step[3][kChunk][TILE::kChannels];          // dt, dt u
   float d[3][kChunk][TILE::kChannels];
   float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
-  float y[2][kChunk][TILE::kChannels + 4], gB[2][kChunk][TILE::kChannels + 4], eA[2][kChunk][TILE::kChannels + 4];   // <C, h>, <g, B>, <e, A>
+  float y[2][kChunk][TILE::kRow], gB[2][kChunk][TILE::kRow], eA[2][kChunk][TILE::kRow];   // <C, h>, <g, B>, <e, A>
   float4 sums[2][kChunk][4][kSumsOfToken * LPC / 4];   // of each warp
-  alignas(16) float skip[TILE::kChannels], bias[TILE::kChannels];
+  alignas(16) float skip[TILE::kChannels], bias[TILE::kChannels];   // (in registers they would be spilled)
 };
 
 // What a backward pass writes beside its results, in the order of the workspace.
@@ -210,13 +210,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
           }
 #pragma unroll
           for (int q = 0; q < kEach; q += 2) {
-            F2 s = add2(f2(dt[q], dt[q + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + q])});
+            F2 s = add2(f2(dt[q], dt[q + 1]), pair_of(&sm.bias[c0 + q]));
             if (a.softplus) s = softplus(s);
-            float x, y, ix, iy;
-            apart(s, x, y), apart(mul2(s, f2(u[q], u[q + 1])), ix, iy);
-            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + q]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float2*>(&sm.d[buf][row][c0 + q]) = there ? make_float2(d[q], d[q + 1]) : make_float2(0.f, 0.f);
+            apart(mul2(s, f2(u[q], u[q + 1])), u[q], u[q + 1]), apart(s, dt[q], dt[q + 1]);
           }
+          put_steps(&sm.step[buf][row][c0], dt, u, me, there);
+          *reinterpret_cast<float4*>(&sm.d[buf][row][c0]) = there ? make_float4(d[0], d[1], d[2], d[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_backward(lasp_scan_args a,
       numbers<T, kEach>(sm.dt[stage][me], dt);
 #pragma unroll
       for (int q = 0; q < kEach; q += 2) {
-        F2 s = add2(f2(dt[q], dt[q + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + q])});
+        F2 s = add2(f2(dt[q], dt[q + 1]), pair_of(&sm.bias[c0 + q]));
         float raw[2], step[2];
         apart(s, raw[0], raw[1]);
         if (a.softplus) s = softplus(s);

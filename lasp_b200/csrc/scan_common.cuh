@@ -21,7 +21,8 @@ struct Tile {
   static constexpr int kGroups = 32 / LPC;            // channels of a warp
   static constexpr int kChannels = 4 * kGroups;
   // units in which a chunk's tokens are brought and prepared: kEach channels of a token, 4 numbers of B or of C
-  static constexpr int kEach = kChannels % 8 ? 2 : 4, kVecs = kChannels / kEach, kUnits = kChunk * kVecs;
+  static constexpr int kEach = 4, kVecs = kChannels / kEach, kUnits = kChunk * kVecs;
+  static constexpr int kRow = kChannels + (LPC == 4 ? 8 : 4);   // of sums that the warps with the states leave: lanes write several rows at once
   static constexpr int kStateUnits = kChunk * LPC;
 };
 // Registers move from the warps that prepare and finish to those that hold the states.  A block is launched with 3 x 128 x kRegisters
@@ -186,6 +187,23 @@ __device__ __forceinline__ S4 rates(const float* A, int n, int states) {
   const float4 v = four_of(A, n, states);
   const auto one = [](float x) { return x *= kLog2e, isinf(x) ? copysignf(3.402823466e38f, x) : x; };
   return {f2(one(v.x), one(v.y)), f2(one(v.z), one(v.w))};
+}
+
+// What a parameter of kEach channels is, zeros where there are none.
+template <typename T, int N>
+__device__ __forceinline__ void params_of(const void* p, bool f32, int channel, int left, float (&out)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) out[k] = p && k < left ? param<T>(p, f32, channel + k) : 0.f;
+}
+// Steps and inputs of a unit's four channels, two 16-byte words: every other four threads write the second word first, so that eight threads
+// together reach every bank.
+__device__ __forceinline__ void put_steps(float2* to, const float (&step)[4], const float (&in)[4], int thread, bool there) {
+  const bool second = thread & 4;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), x = there ? make_float4(step[0], in[0], step[1], in[1]) : zero;
+  const float4 y = there ? make_float4(step[2], in[2], step[3], in[3]) : zero;
+  float4* p = reinterpret_cast<float4*>(to);
+  p[second] = second ? y : x;
+  p[!second] = second ? x : y;
 }
 
 // Which channels a block's tile is: tiles do not reach across groups, the last of a group may be cut short.

@@ -15,8 +15,7 @@ struct Shared {
   Vec<T, 4> B[kStages][TILE::kStateUnits], C[kStages][TILE::kStateUnits];
   float2 step[3][kChunk][TILE::kChannels];                                          // dt, dt u
   float4 B4[3][kChunk][LPC], C4[3][kChunk][LPC];
-  float y[2][kChunk][TILE::kChannels + 4];                                          // <C, h>
-  alignas(16) float skip[TILE::kChannels], bias[TILE::kChannels];
+  float y[2][kChunk][TILE::kRow];                                                   // <C, h>
 };
 
 // wide: u, dt, z, y can be read and written by kEach, B and C by four.
@@ -34,12 +33,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
   if (at.index == at.count) return;
   const int chunks = (at.tokens + kChunk - 1) / kChunk;
   const bool f32 = a.param_dtype == LASP_F32, gated = a.z.data != nullptr, whole = wide && tile.left >= TILE::kChannels;
-  for (int c = threadIdx.x; c < TILE::kChannels; c += kThreads) {
-    const bool there = c < tile.left;
-    sm.skip[c] = there && a.D ? param<T>(a.D, f32, tile.channel + c) : 0.f;
-    sm.bias[c] = there && a.dt_bias ? param<T>(a.dt_bias, f32, tile.channel + c) : 0.f;
-  }
-  __syncthreads();
   const auto rows = [&](const lasp_tokens& t) {
     return static_cast<T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + tile.channel;
   };
@@ -96,6 +89,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
     give_registers<48>();
     static_assert(TILE::kUnits <= kGroup, "a thread has at most one unit of each tensor");
     const int row = me / kVecs, c0 = me % kVecs * kEach;
+    float bias[kEach];
+    params_of<T>(a.dt_bias, f32, tile.channel + c0, tile.left - c0, bias);
     __syncthreads();
     for (int chunk = 0, buf = 0; chunk < chunks + 2; ++chunk, buf = buf == 2 ? 0 : buf + 1) {
       const int stage = chunk % kStages, t0 = chunk * kChunk;
@@ -106,12 +101,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
           numbers<T, kEach>(sm.dt[stage][me], dt), numbers<T, kEach>(sm.u[stage][me], u);
 #pragma unroll
           for (int k = 0; k < kEach; k += 2) {
-            F2 d = add2(f2(dt[k], dt[k + 1]), F2{*reinterpret_cast<const unsigned long long*>(&sm.bias[c0 + k])});
+            F2 d = add2(f2(dt[k], dt[k + 1]), f2(bias[k], bias[k + 1]));
             if (a.softplus) d = softplus(d);
-            float x, y, ix, iy;
-            apart(d, x, y), apart(mul2(d, f2(u[k], u[k + 1])), ix, iy);
-            *reinterpret_cast<float4*>(&sm.step[buf][row][c0 + k]) = there ? make_float4(x, ix, y, iy) : make_float4(0.f, 0.f, 0.f, 0.f);
+            apart(mul2(d, f2(u[k], u[k + 1])), u[k], u[k + 1]), apart(d, dt[k], dt[k + 1]);
           }
+          put_steps(&sm.step[buf][row][c0], dt, u, me, there);
         }
 #pragma unroll
         for (int v = me; v < 2 * TILE::kStateUnits; v += kGroup) {   // (B's and C's for whole warps each)
@@ -128,6 +122,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
     give_registers<48>();
     const int row = me / kVecs, c0 = me % kVecs * kEach, left = tile.left - c0;
     const bool unit = me < TILE::kUnits;
+    float skip[kEach];
+    params_of<T>(a.D, f32, tile.channel + c0, left, skip);
     const T *pu = rows(a.u) + c0, *pdt = rows(a.dt) + c0, *pz = gated ? rows(a.z) + c0 : nullptr;
     const auto state_rows = [&](const lasp_tokens& t) {
       return static_cast<const T*>(t.data) + (int64_t)at.row * t.row_pitch + (int64_t)at.begin * t.token_pitch + (int64_t)tile.group * t.group_pitch;
@@ -161,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_scan_forward(lasp_scan_args a, 
       float y[kEach], u[kEach], z[kEach];
       numbers<T, kEach>(sm.u[stage][me], u);
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) y[k] = fmaf(sm.skip[c0 + k], u[k], sm.y[chunk & 1][row][c0 + k]);
+      for (int k = 0; k < kEach; ++k) y[k] = fmaf(skip[k], u[k], sm.y[chunk & 1][row][c0 + k]);
       if (gated) {
         numbers<T, kEach>(sm.z[stage][me], z);
 #pragma unroll
