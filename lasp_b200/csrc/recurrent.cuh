@@ -223,11 +223,14 @@ struct StepRows {
     if (threadIdx.x < n) slot[threadIdx.x] = slots ? index_at(slots, bits, row0 + threadIdx.x) : row0 + threadIdx.x;
     __syncthreads();
     if (!slots || rows == 1) return;
+    uint32_t seen = 0, comes = 0;
     for (int j = threadIdx.x; j < rows; j += blockDim.x) {
       const int64_t s = index_at(slots, bits, j);
       for (int q = 0; q < n; ++q)
-        if (s == slot[q] && j != row0 + q) atomicOr(j < row0 + q ? &before : &after, 1u << q);
+        if (s == slot[q]) (j < row0 + q ? seen : comes) |= (uint32_t)(j != row0 + q) << q;
     }
+    if (seen) atomicOr(&before, seen);
+    if (comes) atomicOr(&after, comes);
     __syncthreads();
   }
 };

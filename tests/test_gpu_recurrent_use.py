@@ -261,6 +261,60 @@ def test_refusals():
             selective_scan_step(state, *tok, **change)
 
 
+@pytest.mark.parametrize("b,n,c,N", [(1, 5, 1, 1), (2, 1, 3, 2), (1, 17, 2, 3), (1, 1030, 1, 1)])
+def test_the_smallest(b, n, c, N):
+    t, v = scan_inputs(n, F32, b, n, c, N, 1, b), conv_inputs(n, F32, b, n, c, 2, b)
+    t.update(state=None, dstate=None)
+    names = ["y", *[GRADIENTS[k] for k in ("u", "dt", "A", "B", "C", "D", "z", "dt_bias")]]
+    args = dict(softplus=True, cu=None, **t)
+    _close(dict(zip(names, scan_grads(t))), F.scan(**args), F.scan(**args, size=True), 2 * n + 20)
+    args = (v["x"], v["weight"], v["bias"], True, None, None, v["dy"])
+    _close(dict(zip(("y", "dx", "dweight", "dbias"), conv_grads(v))), F.conv(*args), F.conv(*args, size=True), 40)
+
+
+def test_a_batch_that_is_mostly_padding():
+    """600 rows, most of which stand for no sequence and two of which share one."""
+    from lasp_b200 import causal_conv_step, selective_scan_step
+    rows, c, N = 600, 40, 16
+    t, v = scan_inputs(1, F32, rows, 1, c, N, 1, 7), conv_inputs(1, F32, rows, 1, c, 4, 7)
+    tok = {k: t[k][:, 0] if k in ("u", "dt", "B", "C", "z") else t[k] for k in t if t[k] is not None}
+    slots = torch.full((rows,), -1, device=DEV)
+    real = torch.tensor([3, 77, 78, 400, 599], device=DEV)
+    slots[real] = torch.tensor([6, 0, 4, 6, 2], device=DEV)
+    for step, state, args, kw in ((selective_scan_step, t["state"], scan_args(tok), dict(dt_softplus=True)),
+                                  (causal_conv_step, v["state"], (v["x"][:, 0], v["weight"], v["bias"]), dict(activation="silu"))):
+        got, want = state.clone(), state.clone()
+        y = step(got, *args, slots=slots, **kw)
+        small = [a if a is None or a.shape[:1] != (rows,) else a[real] for a in args]
+        assert torch.equal(y[real], step(want, *small, slots=slots[real], **kw)) and torch.equal(got, want)
+        assert not y[slots < 0].any() and torch.equal(got[[1, 3, 5]], state[[1, 3, 5]])
+
+
+def test_traced():
+    """torch.jit.trace: the graph holds the operators themselves."""
+    from lasp_b200 import causal_conv, selective_scan
+    t, v = scan_inputs(2, F32, 1, 30, 16, 16, 1, 1), conv_inputs(2, F32, 1, 30, 16, 4, 1)
+
+    def f(x, dt):
+        u = causal_conv(x, v["weight"], v["bias"], activation="silu")
+        return selective_scan(u, dt, t["A"], t["B"], t["C"], t["D"], t["z"], t["dt_bias"], dt_softplus=True)
+
+    traced = torch.jit.trace(f, (torch.zeros_like(v["x"]), torch.zeros_like(t["dt"])), check_trace=False)
+    assert {"lasp_b200::causal_conv", "lasp_b200::selective_scan"} <= {n.kind() for n in traced.graph.nodes()}
+    assert torch.equal(traced(v["x"], t["dt"]), f(v["x"], t["dt"]))
+
+
+def test_transforms_are_refused():
+    from lasp_b200 import causal_conv, selective_scan
+    t, v = scan_inputs(2, F32, 3, 9, 8, 16, 1, 3), conv_inputs(2, F32, 3, 9, 8, 4, 3)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.vmap(lambda x: causal_conv(x[None], v["weight"]))(v["x"])
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.vmap(lambda u, dt, B, C: selective_scan(u[None], dt[None], t["A"], B[None], C[None]))(t["u"], t["dt"], t["B"], t["C"])
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.grad(lambda x: causal_conv(x, v["weight"]).sum())(v["x"])
+
+
 def test_beyond_32_bits():
     """More than 2^31 numbers: the last tokens of a long row, and the last slots of a large cache."""
     from lasp_b200 import causal_conv, causal_conv_step, selective_scan, selective_scan_step
