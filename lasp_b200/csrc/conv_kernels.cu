@@ -375,7 +375,8 @@ __global__ void __launch_bounds__(256) k_conv_params(lasp_conv_args a, const flo
   }
 }
 
-// Single tokens: the inputs before the next row's token, and that token, are sent for before this row is worked on.
+// Single tokens: the inputs before the next row's token, and that token, are sent for before this row is worked on.  256 rows of 4096 channels, bf16:
+// 10 us (2.6 at the copy rate: a launch and three latencies one after the other, slot, state, output).
 constexpr int kStepThreads = 128;
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(kStepThreads) k_conv_step(lasp_conv_step_args a, int per) {

@@ -5,8 +5,10 @@
 // A block owns a tile of channels of one sequence and walks along its tokens, kChunk at a time.  Four of its warps hold the states: a
 // lane 4 neighbouring ones of one channel, LPC lanes those of a channel (lanes g, g + 32 / LPC, ...: what belongs to a state is then
 // the same for neighbouring lanes, which shared memory serves at once), a warp 32 / LPC channels.  They do nothing but the recurrence and the sums over it:
-// the exponentials bound it (one for every state of every channel and token, 16 per clock and SM), and a warp that also brought, prepared and
-// finished its tokens spent half its time on the latencies of those.  That is what the other eight warps are for.
+// a warp that also brought, prepared and finished its tokens spent half its time on the latencies of those, which is what the other eight
+// warps are for.  What bounds it then is the pipe of shared memory (2 x 2048 x 4096, 16 states, forward: 45 of the 58 clocks that a tile takes
+// for a token where an SM has two blocks) and the chain of the warps that hold the states (68 clocks where it has one); the exponentials, one for every state,
+// channel and token at 16 per clock and SM, take 32.
 #pragma once
 #include <algorithm>
 
