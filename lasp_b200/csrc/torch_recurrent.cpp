@@ -248,7 +248,7 @@ Tensor causal_conv_step(const Tensor& state, const Tensor& x, const Tensor& weig
 }
 
 // ---- scan -------------------------------------------------------------------------------------------------------------------------
-struct ScanInputs {   // laid out as the kernels take them; B and C (batch, tokens, groups, states)
+struct ScanInputs {   // laid out as the kernels take them; B and C (batch, tokens, [groups,] states)
   Tensor u, dt, A, B, C, D, z, bias, state, cu;
   bool softplus;
   int64_t sequences() const { return cu.defined() ? cu.numel() - 1 : u.size(0); }
@@ -258,7 +258,7 @@ struct ScanInputs {   // laid out as the kernels take them; B and C (batch, toke
 lasp_scan_args scan_args(const ScanInputs& s) {
   lasp_scan_args a = {};
   a.rows = (int32_t)s.u.size(0), a.tokens = (int32_t)s.u.size(1), a.channels = (int32_t)s.u.size(2), a.states = (int32_t)s.A.size(1);
-  a.groups = (int32_t)s.B.size(2), a.dtype = lasp_dtype_of(s.u.scalar_type()), a.softplus = s.softplus ? 1 : 0;
+  a.groups = s.B.dim() > 3 ? (int32_t)s.B.size(2) : 1, a.dtype = lasp_dtype_of(s.u.scalar_type()), a.softplus = s.softplus ? 1 : 0;
   const Tensor& p = s.D.defined() ? s.D : s.bias;
   a.param_dtype = p.defined() ? lasp_dtype_of(p.scalar_type()) : LASP_F32;
   a.sequences = s.cu.defined() ? (int32_t)s.cu.numel() - 1 : 0, a.index_bits = bits_of(s.cu), a.offsets = data_of(s.cu);
@@ -302,7 +302,7 @@ class Scan : public torch::autograd::Function<Scan> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({u, dt, A, B, C, D.value_or(Tensor()), z.value_or(Tensor()), bias.value_or(Tensor()), cu.value_or(Tensor()), out[2]});
     ctx->saved_data["u"] = u.sizes().vec();
-    ctx->saved_data["B"] = B.sizes().vec();
+    ctx->saved_data["B"] = B.sizes().vec(), ctx->saved_data["C"] = C.sizes().vec();
     ctx->saved_data["sequences"] = have(cu) ? cu->numel() : 0;
     ctx->saved_data["kept"] = out[2].numel();
     ctx->saved_data["type"] = (int64_t)u.scalar_type();
@@ -319,10 +319,10 @@ class Scan : public torch::autograd::Function<Scan> {
     variable_list out(12);
     const Tensor d_state = grads.size() > 1 ? grads[1] : Tensor();
     if (!grads[0].defined() && !d_state.defined()) return out;
-    const auto sizes = ctx->saved_data["u"].toIntVector(), bsizes = ctx->saved_data["B"].toIntVector();
+    const auto sizes = ctx->saved_data["u"].toIntVector(), bsizes = ctx->saved_data["B"].toIntVector(), csizes = ctx->saved_data["C"].toIntVector();
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt(), ptype = (at::ScalarType)ctx->saved_data["param_type"].toInt();
     const at::Device device(at::kCUDA, (c10::DeviceIndex)ctx->saved_data["device"].toInt());
-    const int64_t cu_count = ctx->saved_data["sequences"].toInt(), channels = sizes[2], states = bsizes[3];
+    const int64_t cu_count = ctx->saved_data["sequences"].toInt(), channels = sizes[2], states = bsizes.back();
     const c10::cuda::CUDAGuard guard(device);
     const auto param = [&](const Tensor& t, const char* name) { return t.defined() ? Maybe(saved(t, name, {channels}, ptype, device)) : Maybe(); };
     Maybe cu;
@@ -333,7 +333,7 @@ class Scan : public torch::autograd::Function<Scan> {
     }
     const ScanInputs s = laid_out(saved(in[0], "u", sizes, type, device), saved(in[1], "dt", sizes, type, device),
                                   saved(in[2], "A", {channels, states}, at::kFloat, device), saved(in[3], "B", bsizes, type, device),
-                                  saved(in[4], "C", bsizes, type, device), param(in[5], "D"),
+                                  saved(in[4], "C", csizes, type, device), param(in[5], "D"),
                                   in[6].defined() ? Maybe(saved(in[6], "z", sizes, type, device)) : Maybe(), param(in[7], "dt_bias"), Maybe(), cu,
                                   ctx->saved_data["softplus"].toBool());
     const Tensor kept = saved(in[9], "of the kept states", {ctx->saved_data["kept"].toInt()}, at::kByte, device).contiguous();
@@ -372,13 +372,18 @@ void check_scan_params(const Tensor& u, const Tensor& A, const Maybe& D, const M
   if (have(D)) check_param("D", *D, u, {c});
   if (have(bias)) check_param("dt_bias", *bias, u, {c});
 }
-// B and C with their groups: (..., states) is one group
-Tensor grouped(const char* name, const Tensor& t, const Tensor& u, int64_t states) {
+// How many groups of channels B or C has: (..., states) is one
+int64_t groups_of(const char* name, const Tensor& t, const Tensor& u, int64_t states) {
   TORCH_CHECK_VALUE((t.dim() == u.dim() || t.dim() == u.dim() + 1) && t.sizes().slice(0, u.dim() - 1) == u.sizes().slice(0, u.dim() - 1) && t.size(-1) == states,
                     name, " has shape ", t.sizes(), "; expected (", u.sizes().slice(0, u.dim() - 1), ", [groups,] ", states, " states)");
-  if (t.dim() == u.dim()) return t.unsqueeze(-2);
+  check_of(name, t, u, t.sizes());
+  if (t.dim() == u.dim()) return 1;
   TORCH_CHECK_VALUE(t.size(-2) >= 1 && t.size(-2) <= 65535 && u.size(-1) % t.size(-2) == 0, name, " has ", t.size(-2), " groups, which must divide ", u.size(-1), " channels");
-  return t;
+  return t.size(-2);
+}
+void check_groups(const Tensor& B, const Tensor& C, const Tensor& u, int64_t states) {
+  const int64_t of_B = groups_of("B", B, u, states), of_C = groups_of("C", C, u, states);
+  TORCH_CHECK_VALUE(of_B == of_C, "C has ", of_C, " groups, B has ", of_B);
 }
 
 std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Maybe& D,
@@ -387,9 +392,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& dt, con
   check_plain("u", u, u);
   check_of("dt", dt, u, u.sizes());
   check_scan_params(u, A, D, bias);
-  const Tensor Bg = grouped("B", B, u, A.size(1)), Cg = grouped("C", C, u, A.size(1));
-  check_of("B", Bg, u, Bg.sizes());
-  check_of("C", Cg, u, Bg.sizes());
+  check_groups(B, C, u, A.size(1));
   if (have(z)) check_of("z", *z, u, u.sizes());
   const int64_t sequences = check_sequences(cu, u);
   if (have(state)) check_state("initial_state", *state, u, at::kFloat, {sequences, u.size(2), A.size(1)});
@@ -402,9 +405,9 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& dt, con
   }
   variable_list out;
   if (graph)
-    out = Scan::apply(u, dt, A, Bg, Cg, skip, z, b, state, cu, softplus, want_state);
+    out = Scan::apply(u, dt, A, B, C, skip, z, b, state, cu, softplus, want_state);
   else
-    out = run_scan(Scan::laid_out(u, dt, A, Bg, Cg, skip, z, b, state, cu, softplus), want_state, false);
+    out = run_scan(Scan::laid_out(u, dt, A, B, C, skip, z, b, state, cu, softplus), want_state, false);
   return {out[0], want_state ? out[1] : Tensor()};
 }
 
@@ -414,9 +417,7 @@ Tensor selective_scan_step(const Tensor& state, const Tensor& u, const Tensor& d
   check_plain("u", u, u);
   check_of("dt", dt, u, u.sizes());
   check_scan_params(u, A, D, bias);
-  const Tensor Bg = side_by_side(grouped("B", B, u, A.size(1))), Cg = side_by_side(grouped("C", C, u, A.size(1)));
-  check_of("B", Bg, u, Bg.sizes());
-  check_of("C", Cg, u, Bg.sizes());
+  check_groups(B, C, u, A.size(1));
   if (have(z)) check_of("z", *z, u, u.sizes());
   TORCH_CHECK_VALUE(state.dim() == 3, "state has shape ", state.sizes(), "; expected (slots, channels, states)");
   check_state("state", state, u, at::kFloat, {state.size(0), u.size(1), A.size(1)});
@@ -429,13 +430,13 @@ Tensor selective_scan_step(const Tensor& state, const Tensor& u, const Tensor& d
   const bool plain = have(D) ? as_inputs(u, *D, bias) : have(bias) && bias->scalar_type() == u.scalar_type();
   const auto param = [&](const Maybe& t) { return have(t) ? (plain ? *t : in_fp32(*t)).contiguous() : Tensor(); };
   const Tensor us = side_by_side(u), dts = side_by_side(dt), As = A.contiguous(), skip = param(D), b = param(bias), named = contiguous(slots);
-  const Tensor zs = have(z) ? side_by_side(*z) : Tensor();
+  const Tensor zs = have(z) ? side_by_side(*z) : Tensor(), Bs = side_by_side(B), Cs = side_by_side(C);
   lasp_scan_step_args a = {};
-  a.rows = (int32_t)u.size(0), a.channels = (int32_t)u.size(1), a.states = (int32_t)A.size(1), a.groups = (int32_t)Bg.size(1);
+  a.rows = (int32_t)u.size(0), a.channels = (int32_t)u.size(1), a.states = (int32_t)A.size(1), a.groups = Bs.dim() > 2 ? (int32_t)Bs.size(1) : 1;
   const Tensor& p = skip.defined() ? skip : b;
   a.dtype = lasp_dtype_of(u.scalar_type()), a.param_dtype = p.defined() ? lasp_dtype_of(p.scalar_type()) : LASP_F32, a.softplus = softplus ? 1 : 0;
   a.slot_count = (int32_t)state.size(0), a.index_bits = bits_of(named), a.slots = data_of(named);
-  a.u = rows_of(us), a.dt = rows_of(dts), a.z = rows_of(zs), a.B = rows_of(Bg), a.C = rows_of(Cg), a.y = rows_of(y);
+  a.u = rows_of(us), a.dt = rows_of(dts), a.z = rows_of(zs), a.B = rows_of(Bs), a.C = rows_of(Cs), a.y = rows_of(y);
   a.A = As.const_data_ptr<float>(), a.D = data_of(skip), a.dt_bias = data_of(b), a.state = state.data_ptr<float>();
   Range range("lasp_b200_scan_step");
   check_status("lasp_b200_scan_step", lasp_b200_scan_step(&a, at::cuda::getCurrentCUDAStream().stream()));
