@@ -232,8 +232,8 @@ int tiles_of(int channels, int groups) {
 // the tokens (scan_parts.cu) finds those.  It takes the exponentials once more, so segments come only where they are that many.
 constexpr int kParts = 4, kUncut = 0x7ffffff0;
 // Tokens of a segment; segments for which the first pass pays, forward and backward.  us without and with, bf16, 16 states: 4096 tokens of
-// 1024 channels 157 and 69, 602 and 169; 16384 of 4096 (two segments) 612 and 933, 2418 and 2085; three forward 613 and 653.
-constexpr int kLeast = 128, kLeastForward = 4, kLeastBack = 2;
+// 1024 channels 157 and 64, 602 and 143; 16384 of 2560 (three segments) 591 and 499, 2383 and 1226; of 4096 (two) 592 and 739, 2418 and 1842.
+constexpr int kLeast = 128, kLeastForward = 3, kLeastBack = 2;
 struct Cuts {
   int length, part;       // tokens of a segment, of a part: multiples of kChunk, or kUncut
   int64_t slots, parts;   // how many there may be
@@ -340,8 +340,10 @@ int64_t floats_of(const Cuts& c, int tiles) { return c.length == kUncut ? 0 : c.
 template <class TILE>
 Cuts cuts_of(const lasp_scan_args& a, int tiles, bool backward, float* ws) {
   Cuts c{kUncut, kUncut, 0, 0, nullptr, nullptr};
-  // two blocks an SM, no more (sequences of a packed row: as many tokens for each as if there were one)
-  const int64_t unit = kParts * kChunk, segments = 2 * std::max(1, sm_count()) / ((int64_t)tiles * a.rows);
+  // two blocks an SM, no more (sequences of a packed row: as many tokens for each as if there were one); back three segments, too, where whole
+  // sequences leave most SMs one block and some two: those are then 2/3 as long (192 blocks, 1000 tokens of 32 states: 215 us without, 191 with)
+  const int64_t unit = kParts * kChunk, blocks = (int64_t)tiles * a.rows, sms = std::max(1, sm_count());
+  const int64_t segments = backward && blocks > sms && 3 * blocks <= 4 * sms ? 3 : 2 * sms / blocks;
   if (segments >= 2) {
     const int64_t length = std::max<int64_t>(kLeast, ((a.tokens + segments - 1) / segments + unit - 1) / unit * unit);
     if (a.tokens > (backward ? kLeastBack - 1 : kLeastForward - 1) * length) c.length = (int)length, c.part = c.length / kParts;
