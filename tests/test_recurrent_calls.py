@@ -132,6 +132,16 @@ def test_scan_c_checks_of_one_pass():
         assert lib.lasp_b200_scan_backward(C.byref(scan_args(**kw)), None) == status
 
 
+def test_scan_c_checks_of_the_forward_workspace():
+    """A long sequence of few channels is cut into segments, which takes a workspace; a short one takes none."""
+    lib = _cabi.load()
+    need = lambda **kw: lib.lasp_b200_scan_forward_workspace_bytes(C.byref(scan_args(**kw)))   # noqa: E731
+    assert need(rows=1, tokens=4096) > 0 and need(rows=1, tokens=100) == 0 and need(rows=1, tokens=4096, states=0) == 0 and need(rows=1, tokens=0) == 0
+    for kw, status in ((dict(ws=None), -1), (dict(ws=P + 4), -4), (dict(ws_bytes=8), -5)):
+        kw = {**dict(rows=1, tokens=4096, kept=None, ws=P, ws_bytes=need(rows=1, tokens=4096)), **kw}
+        assert lib.lasp_b200_scan_forward(C.byref(scan_args(**kw)), None) == status
+
+
 def test_step_c_checks():
     lib = _cabi.load()
 
