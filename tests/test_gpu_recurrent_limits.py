@@ -1,0 +1,42 @@
+"""causal_conv, selective_scan and their steps at the limits."""
+import pytest
+import torch
+
+from tests.test_gpu_recurrent import BF16, DEV, F16, F32
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- large values --------------------------------------------------------------------------------------------------------------
+LARGE = [0.0, 1.0, 4.0, 15.0, 30.0, 88.0, 1e4, 2.0 ** 24 - 1, 2.0 ** 24 + 2, 2.0 ** 24 + 4, 2.0 ** 25, 1e9, 1e30]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("c_odd", [False, True])
+@pytest.mark.parametrize("n", [1, 64])
+def test_silu_derivative_of_large_inputs(dtype, c_odd, n):
+    """The derivative s (1 + p (1 - s)) is one for every large p and zero for every large -p.  With one tap of 1 in a row of equal
+    inputs p is the input, so that dx, and of a single token every gradient, is the derivative itself."""
+    from lasp_b200 import causal_conv
+    p = torch.tensor([s * v for v in LARGE for s in (1, -1) if v <= torch.finfo(dtype).max] + [2.0] * c_odd, device=DEV).to(dtype)
+    c, width = p.numel(), 4
+    x = p.expand(1, n, c).contiguous().requires_grad_(True)
+    weight = torch.zeros(c, width, device=DEV)
+    weight[:, -1] = 1
+    if n == 1:   # (behind a state of zeros the other taps count for the gradients alone)
+        weight[:] = 1
+    weight.requires_grad_(True)
+    bias, state = torch.zeros(c, device=DEV, requires_grad=True), torch.zeros(1, width - 1, c, dtype=dtype, device=DEV, requires_grad=True)
+    y = causal_conv(x, weight, bias, activation="silu", initial_state=state)
+    dx, dw, db, ds = torch.autograd.grad(y, [x, weight, bias, state], torch.ones_like(y))
+    v = p.double()
+    s = torch.sigmoid(v)
+    want = s * (1 + v * (1 - s))
+    # s is off by 2^-22 and by |p| 2^-23 of itself (the exponent's rounding), 1 - s by 2^-22 until it is exact, from 18 on
+    room = (4 + 3 * v.abs().clamp(max=18)) * 2.0 ** -22
+    half = torch.finfo(dtype).eps / 2
+    assert ((dx[0].double() - want).abs() <= room + half * want.abs()).all(), (dx[0].double() - want).abs().max()
+    assert ((db.double() / n - want).abs() <= room + n * 2.0 ** -24).all()
+    if n == 1:
+        assert ((dw[:, -1].double() - v * want).abs() <= v.abs() * (room + 2.0 ** -24)).all() and not dw[:, :-1].any()
+        assert ((ds[0].double() - want).abs() <= room + half * want.abs()).all()
