@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kVecs* kRuns, 4) k_conv_backward(lasp_conv_arg
           F2 full[W];
 #pragma unroll
           for (int m = 0; m < W - 1; ++m) full[m] = reach >= W - 1 - m ? fma2(taps.w[m].p[k], d.p[k], sum[m].p[k]) : sum[m].p[k];
-          full[W - 1] = mul2(taps.w[W - 1].p[k], d.p[k]);
+          full[W - 1] = inside ? mul2(taps.w[W - 1].p[k], d.p[k]) : f2(0.f, 0.f);   // (no product: a weight may be infinite)
           out.p[k] = full[0];
 #pragma unroll
           for (int m = 0; m < W - 1; ++m) sum[m].p[k] = full[m + 1];

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_recurrent import BF16, DEV, F16, F32
+from tests.test_gpu_recurrent import BF16, DEV, F16, F32, _cu, conv_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,18 @@ def test_silu_derivative_of_large_inputs(dtype, c_odd, n):
     if n == 1:
         assert ((dw[:, -1].double() - v * want).abs() <= v.abs() * (room + 2.0 ** -24)).all() and not dw[:, :-1].any()
         assert ((ds[0].double() - want).abs() <= room + half * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_infinite_weights_and_tokens_outside_the_sequences(dtype):
+    """Tokens that lie in no sequence get zeros, whatever the weights are."""
+    from lasp_b200 import causal_conv
+    t = conv_inputs(9, dtype, 1, 60, 24, 4, 2)
+    weight = t["weight"].clone()
+    weight[::2] = float("inf")
+    leaf = [v.requires_grad_(True) for v in (t["x"].clone(), weight, t["bias"].clone())]
+    y = causal_conv(*leaf, cu_seqlens=_cu([7, 30, 41]))
+    dx = torch.autograd.grad(y, leaf, t["dy"])[0]
+    for v in (y, dx):
+        assert not v[:, :7].any() and not v[:, 41:].any()
+        assert v[:, 7:41, 1::2].isfinite().all()
