@@ -335,7 +335,7 @@ LASP_B200_API int lasp_b200_forward_static(const lasp_problem* p, const lasp_fwd
  * (No counterpart in the reference.)  Tensors of tokens are addressed by pitches, in elements, with the channels (or states)
  * of a token side by side: element (row, token, group, i) lies at data + row * row_pitch + token * token_pitch + group *
  * group_pitch + i.  Nothing else is asked of their alignment than that of their type; where addresses and pitches are
- * multiples of 16 bytes loads are wider.
+ * multiples of 16 bytes loads are wider.  At most 2147480000 tokens and as many channels (LASP_ERR_TOO_LARGE).
  *
  * Sequences: with sequences = 0 every row is one, of `tokens` tokens.  Otherwise rows is 1 and the row is packed: sequence i is
  * tokens offsets[i] to offsets[i + 1] (device, ascending, index_bits 32 or 64 each; out of range they are clamped), an empty one

@@ -4,7 +4,7 @@
 namespace {
 
 constexpr int64_t kMostBlocks = 2147483647;
-constexpr int kMostTokens = 2147480000;   // (a run or chunk beyond is still an int)
+constexpr int kMostTokens = 2147480000, kMostChannels = kMostTokens;   // (a run, chunk or tile beyond is still an int)
 
 bool known(int dtype) { return dtype == LASP_F32 || dtype == LASP_BF16 || dtype == LASP_F16; }
 bool params_ok(int dtype, int param_dtype) { return param_dtype == LASP_F32 || param_dtype == dtype; }
@@ -17,7 +17,7 @@ int check_conv(const lasp_conv_args* a) {
   if (a->rows <= 0 || a->tokens < 0 || a->channels <= 0 || a->width < 2 || a->width > 4 || a->sequences < 0) return LASP_ERR_SHAPE;
   if (a->activation != LASP_ACT_NONE && a->activation != LASP_ACT_SILU) return LASP_ERR_SHAPE;
   if (a->sequences && (a->rows != 1 || !bits_ok(a->offsets, a->index_bits))) return LASP_ERR_SHAPE;
-  if (a->rows > 65535 || a->sequences > (1 << 17) || a->tokens > kMostTokens) return LASP_ERR_TOO_LARGE;
+  if (a->rows > 65535 || a->sequences > (1 << 17) || a->tokens > kMostTokens || a->channels > kMostChannels) return LASP_ERR_TOO_LARGE;
   if (!a->weight || (a->sequences && !a->offsets) || (a->tokens && missing(a->x))) return LASP_ERR_NULL;
   return LASP_OK;
 }
@@ -30,7 +30,9 @@ int check_scan(const lasp_scan_args* a) {
   if (a->sequences && (a->rows != 1 || !bits_ok(a->offsets, a->index_bits))) return LASP_ERR_SHAPE;
   // (a block for every eight channels of every sequence at most; a thread for every dB and dC of a group)
   const int64_t sequences = a->sequences ? (int64_t)a->sequences + 1 : a->rows;
-  if (a->tokens > kMostTokens || sequences * (a->channels / 8 + a->groups) > kMostBlocks || (int64_t)a->rows * a->tokens / 2 > kMostBlocks) return LASP_ERR_TOO_LARGE;
+  if (a->tokens > kMostTokens || a->channels > kMostChannels || sequences * (a->channels / 8 + a->groups) > kMostBlocks ||
+      (int64_t)a->rows * a->tokens / 2 > kMostBlocks)
+    return LASP_ERR_TOO_LARGE;
   if (!a->A || (a->sequences && !a->offsets)) return LASP_ERR_NULL;
   if (a->tokens && (missing(a->u) || missing(a->dt) || missing(a->B) || missing(a->C))) return LASP_ERR_NULL;
   return LASP_OK;
@@ -91,7 +93,7 @@ int lasp_b200_conv_step(const lasp_conv_step_args* a, void* stream) {
   if (!known(a->dtype) || !params_ok(a->dtype, a->param_dtype)) return LASP_ERR_DTYPE;
   if (a->rows <= 0 || a->channels <= 0 || a->width < 2 || a->width > 4 || a->slot_count < 0 || !bits_ok(a->slots, a->index_bits)) return LASP_ERR_SHAPE;
   if (a->activation != LASP_ACT_NONE && a->activation != LASP_ACT_SILU) return LASP_ERR_SHAPE;
-  if (a->rows > 65535) return LASP_ERR_TOO_LARGE;
+  if (a->rows > 65535 || a->channels > kMostChannels) return LASP_ERR_TOO_LARGE;
   if (!a->weight || missing(a->x) || missing(a->y) || (a->slot_count && !a->state)) return LASP_ERR_NULL;
   return lasp::status_of(lasp::conv_step(*a, static_cast<cudaStream_t>(stream)));
 }
@@ -101,7 +103,7 @@ int lasp_b200_scan_step(const lasp_scan_step_args* a, void* stream) {
   if (!known(a->dtype) || !params_ok(a->dtype, a->param_dtype)) return LASP_ERR_DTYPE;
   if (a->rows <= 0 || a->channels <= 0 || a->states <= 0 || a->states > 64 || a->slot_count < 0 || !bits_ok(a->slots, a->index_bits)) return LASP_ERR_SHAPE;
   if (a->groups <= 0 || a->channels % a->groups) return LASP_ERR_SHAPE;
-  if (a->rows > 65535) return LASP_ERR_TOO_LARGE;
+  if (a->rows > 65535 || a->channels > kMostChannels) return LASP_ERR_TOO_LARGE;
   if (!a->A || missing(a->u) || missing(a->dt) || missing(a->B) || missing(a->C) || missing(a->y) || (a->slot_count && !a->state)) return LASP_ERR_NULL;
   return lasp::status_of(lasp::scan_step(*a, static_cast<cudaStream_t>(stream)));
 }

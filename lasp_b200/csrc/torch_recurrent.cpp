@@ -53,16 +53,17 @@ int64_t check_sequences(const Maybe& cu, const Tensor& x) {   // how many sequen
   TORCH_CHECK_VALUE(cu->numel() >= 2, "cu_seqlens holds where each sequence begins and where the last one ends; got ", cu->numel(), " numbers");
   return cu->numel() - 1;
 }
+constexpr int64_t kMost = 2147480000;   // tokens, channels
 void check_tokens(const char* name, const Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() == 3, name, " has shape ", x.sizes(), "; expected (batch, tokens, channels)");
   lasp_dtype_of(x.scalar_type());
   TORCH_CHECK_VALUE(x.size(2) > 0, name, " has no channels");
-  TORCH_CHECK_VALUE(x.size(1) <= 2147480000 && x.size(2) <= INT32_MAX && x.size(0) <= INT32_MAX, name, " of shape ", x.sizes(), " is too large");
+  TORCH_CHECK_VALUE(x.size(1) <= kMost && x.size(2) <= kMost && x.size(0) <= INT32_MAX, name, " of shape ", x.sizes(), " is too large");
 }
 void check_step(const char* name, const Tensor& x) {
   TORCH_CHECK_VALUE(x.dim() == 2, name, " has shape ", x.sizes(), "; expected (batch, channels): one token of every row");
   lasp_dtype_of(x.scalar_type());
-  TORCH_CHECK_VALUE(x.size(1) > 0 && x.size(1) <= INT32_MAX, name, " has ", x.size(1), " channels");
+  TORCH_CHECK_VALUE(x.size(1) > 0 && x.size(1) <= kMost, name, " has ", x.size(1), " channels");
   TORCH_CHECK_VALUE(x.size(0) <= 65535, "a step of ", x.size(0), " rows exceeds 65535");
 }
 void check_slots(const Maybe& slots, const Tensor& x, const Tensor& state) {

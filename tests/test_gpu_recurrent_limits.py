@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_recurrent import BF16, DEV, F16, F32, _cu, conv_inputs
+from tests.test_gpu_recurrent import BF16, DEV, F16, F32, _cu, _normal, conv_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,18 @@ def test_infinite_weights_and_tokens_outside_the_sequences(dtype):
     for v in (y, dx):
         assert not v[:, :7].any() and not v[:, 41:].any()
         assert v[:, 7:41, 1::2].isfinite().all()
+
+
+# ---- more than 2^31 numbers ----------------------------------------------------------------------------------------------------
+def test_weights_beyond_32_bits():
+    """Taps and a bias of more than 2^31 numbers together."""
+    from lasp_b200 import causal_conv
+    c = 429_500_000
+    assert 5 * c >= 2 ** 31
+    x = torch.ones(1, 1, c, dtype=BF16, device=DEV)
+    x[..., -1000:] = _normal(torch.Generator(device=DEV).manual_seed(0), 1000).to(BF16)
+    w = torch.zeros(c, 4, dtype=BF16, device=DEV).requires_grad_(True)
+    bias = torch.zeros(c, dtype=BF16, device=DEV).requires_grad_(True)
+    dw, db = torch.autograd.grad(causal_conv(x, w, bias), [w, bias], x)
+    assert torch.equal(db, x[0, 0]) and not dw[:, :3].any()
+    assert torch.equal(dw[:, 3], (x[0, 0].float() ** 2).to(BF16))
