@@ -37,6 +37,7 @@ thread_local char g_cuda_error[256] = "";
 
 int lasp::status_of(cudaError_t err) {
   if (err == cudaSuccess) return LASP_OK;
+  cudaGetLastError();   // (reported here: the next launch would take it for its own)
   snprintf(g_cuda_error, sizeof(g_cuda_error), "%s%s%s", cudaGetErrorString(err),
            lasp::g_failed_step[0] ? " in " : "", lasp::g_failed_step);
   lasp::g_failed_step = "";

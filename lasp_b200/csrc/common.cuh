@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "lasp_b200.h"
+#include "per_device.h"
 
 namespace lasp {
 
@@ -97,16 +98,12 @@ extern thread_local const char* g_failed_step;
 // the attribute call costs the host about as much as a launch.
 template <auto fn>
 cudaError_t opt_in_smem(size_t bytes) {
-  static bool done[64] = {};
+  static PerDevice asked;
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess && dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
   if (err == cudaSuccess)
-    err = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (err != cudaSuccess)
-    g_failed_step = "cudaFuncSetAttribute(max dynamic shared memory)";
-  else if (dev >= 0 && dev < 64)
-    done[dev] = true;
+    err = asked.once(dev, [bytes] { return cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); });
+  if (err != cudaSuccess) g_failed_step = "cudaFuncSetAttribute(max dynamic shared memory)";
   return err;
 }
 

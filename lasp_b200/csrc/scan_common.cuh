@@ -39,15 +39,21 @@ __device__ __forceinline__ void give_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 // Shared memory and, because a warp that takes more registers than there are waits for good, the registers that a kernel is launched with:
-// looked at once for each kernel and device.
+// looked at until both are as they should be, once for each kernel and device.
 template <auto kernel>
 cudaError_t ready(size_t smem) {
-  static const cudaError_t launched_with = [] {
-    cudaFuncAttributes at;
-    const cudaError_t err = cudaFuncGetAttributes(&at, (const void*)kernel);
-    return err != cudaSuccess ? err : at.numRegs >= kRegisters ? cudaSuccess : cudaErrorInvalidConfiguration;
-  }();
-  return launched_with != cudaSuccess ? launched_with : opt_in_smem<kernel>(smem);
+  static PerDevice looked;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess)
+    err = looked.once(dev, [] {
+      cudaFuncAttributes at;
+      const cudaError_t e = cudaFuncGetAttributes(&at, (const void*)kernel);
+      return e != cudaSuccess ? e : at.numRegs >= kRegisters ? cudaSuccess : cudaErrorInvalidConfiguration;
+    });
+  if (err == cudaSuccess) return opt_in_smem<kernel>(smem);
+  g_failed_step = "cudaFuncGetAttributes(registers of a scan kernel)";
+  return err;
 }
 
 // `BYTES` (4, 8, 16 or 32) from global to shared memory without a register in between.
