@@ -138,10 +138,10 @@ __device__ __forceinline__ F2 sigmoid(F2 p) {
   return f2(reciprocal(x), reciprocal(y));
 }
 __device__ __forceinline__ F2 silu(F2 p) { return mul2(p, sigmoid(p)); }
-// s + s (p (1 - s)): 1 - s before it meets p, which may be so large that p + 1 is no fp32 number any more
+// s + (s p - s (s p)): the difference, exactly zero where s is one, before the sum, since p may be so large that p + 1 is no fp32 number any more
 __device__ __forceinline__ F2 d_silu(F2 p) {
-  const F2 s = sigmoid(p), rest = fma2(s, f2(-1.f, -1.f), f2(1.f, 1.f));
-  return fma2(s, mul2(p, rest), s);
+  const F2 s = sigmoid(p), sp = mul2(s, p);
+  return add2(s, fma2(mul2(s, f2(-1.f, -1.f)), sp, sp));
 }
 
 // V neighbouring channels as pairs; of a single channel the other half is zero.
