@@ -353,20 +353,20 @@ __global__ void __launch_bounds__(kVecs* kRuns, 4) k_conv_backward(lasp_conv_arg
   }
 }
 
-// dweight, dbias: the partial sums in the order of their blocks
+// dweight, dbias: the partial sums in the order of their blocks.  blockIdx.y: the tap, or the bias.
 template <typename T>
 __global__ void __launch_bounds__(256) k_conv_params(lasp_conv_args a, const float* partial, int parts) {
   __shared__ float part[8][32];
-  const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x, all = (int64_t)(a.width + 1) * a.channels;
+  const int c = blockIdx.x * 32 + threadIdx.x, k = blockIdx.y;
+  const int64_t all = (int64_t)(a.width + 1) * a.channels, i = (int64_t)k * a.channels + c;
   float s = 0.f;
-  if (i < all)
+  if (c < a.channels)
     for (int p = threadIdx.y; p < parts; p += 8) s += partial[p * all + i];
   part[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y || i >= all) return;
+  if (threadIdx.y || c >= a.channels) return;
 #pragma unroll
   for (int r = 1; r < 8; ++r) s += part[r][threadIdx.x];
-  const int k = (int)(i / a.channels), c = (int)(i - (int64_t)k * a.channels);
   const bool f32 = a.param_dtype == LASP_F32;
   if (k < a.width) {
     if (a.dweight) store_param<T>(a.dweight, f32, (int64_t)c * a.width + k, s);
@@ -469,7 +469,7 @@ cudaError_t backward_as(const lasp_conv_args& a, cudaStream_t st) {
   const bool params = a.dweight || a.dbias;
   float* partial = params ? static_cast<float*>(a.ws) : nullptr;
   if (blocks + extra) k_conv_backward<T, V, W><<<grid, dim3(kVecs, kRuns), 0, st>>>(a, run, blocks, partial);
-  if (params) k_conv_params<T><<<(unsigned)(((int64_t)(W + 1) * a.channels + 31) / 32), dim3(32, 8), 0, st>>>(a, partial, blocks * a.rows);
+  if (params) k_conv_params<T><<<dim3((a.channels + 31) / 32, W + 1), dim3(32, 8), 0, st>>>(a, partial, blocks * a.rows);
   return cudaGetLastError();
 }
 
