@@ -373,10 +373,12 @@ Plan plan_as(const lasp_scan_args& a) {
   using TILE = Tile<LPC>;
   Plan p;
   p.tiles = tiles_of<TILE>(a.channels, a.groups);
-  const Cuts cuts = cuts_of<TILE>(a, p.tiles, true, nullptr);
+  // 90 KB of shared memory for 16-bit types, 115 (fp32, 16 states), 109 (32), 132 and 157 (64 states, 16 bits and fp32)
+  const int resident = blocks_of_sm(a.dtype == LASP_F32 ? sizeof(Shared<float, LPC>) : sizeof(Shared<__half, LPC>));
+  const Cuts cuts = cuts_of<TILE>(a, p.tiles, true, resident, nullptr);
   p.tokens = (size_t)p.tiles * a.rows * a.tokens * 8 * LPC;
   p.rates = (size_t)cuts.slots * p.tiles * kGroup * 4, p.skips = ((size_t)cuts.slots * 2 * a.channels + 3) / 4 * 4, p.parts = (size_t)floats_of<TILE>(cuts, p.tiles);
-  p.cuts = cuts_of<TILE>(a, p.tiles, true, static_cast<float*>(a.ws) + p.tokens + p.rates + p.skips);
+  p.cuts = cuts_of<TILE>(a, p.tiles, true, resident, static_cast<float*>(a.ws) + p.tokens + p.rates + p.skips);
   return p;
 }
 

@@ -28,7 +28,7 @@ struct Tile {
   static constexpr int kStateUnits = kChunk * LPC;
 };
 // Registers move from the warps that prepare and finish to those that hold the states.  A block is launched with 3 x 128 x kRegisters
-// (two blocks an SM); the shares add up to no more.
+// (two blocks an SM, where shared memory allows it); the shares add up to no more.
 constexpr int kRegisters = 80;
 template <int N>
 __device__ __forceinline__ void take_registers() {
@@ -237,9 +237,13 @@ int tiles_of(int channels, int groups) {
 // segment, do to a state of zero (`ends`) and from the sums of their steps, whose exponentials are the parts' decays: a first pass over
 // the tokens (scan_parts.cu) finds those.  It takes the exponentials once more, so segments come only where they are that many.
 constexpr int kParts = 4, kUncut = 0x7ffffff0;
-// Tokens of a segment; segments for which the first pass pays, forward and backward.  us without and with, bf16, 16 states: 4096 tokens of
-// 1024 channels 157 and 64, 602 and 143; 16384 of 2560 (three segments) 591 and 499, 2383 and 1226; of 4096 (two) 592 and 739, 2418 and 1842.
-constexpr int kLeast = 128, kLeastForward = 3, kLeastBack = 2;
+// Tokens of a segment; segments for which the first pass pays: two backward where an SM has two blocks, else three.  us of whole rows and of rows in
+// segments, 16384 tokens of 4096 channels and 16 states (128 blocks): forward 600 and 793 (two); backward 2314 and 1978 (two) in bf16, in fp32,
+// where an SM has one block, 2283 and 2416 (two: as long as whole rows, and the first pass).  In three (4096 tokens in 80 blocks): forward 160 and 142,
+// backward, one block an SM, 553 and 414 (fp32, 16 states), 574 and 468 (bf16, 64).
+constexpr int kLeast = 128, kLeastSegments = 3, kLeastOfTwoBlocks = 2;
+// Blocks of an SM: it has 228 KB of shared memory, of which a block takes 1 KB more than it asks for.
+constexpr int blocks_of_sm(size_t smem) { return 2 * (smem + 1024) <= 228 * 1024 ? 2 : 1; }
 struct Cuts {
   int length, part;       // tokens of a segment, of a part: multiples of kChunk, or kUncut
   int64_t slots, parts;   // how many there may be
@@ -343,16 +347,21 @@ __device__ void fill_outside(const lasp_scan_args& a, const lasp_tokens& y, cons
 // Floats that the parts' ends and steps take.
 template <class TILE>
 int64_t floats_of(const Cuts& c, int tiles) { return c.length == kUncut ? 0 : c.parts * tiles * (4 * kGroup + TILE::kChannels); }
+// resident: blocks of an SM
 template <class TILE>
-Cuts cuts_of(const lasp_scan_args& a, int tiles, bool backward, float* ws) {
+Cuts cuts_of(const lasp_scan_args& a, int tiles, bool backward, int resident, float* ws) {
   Cuts c{kUncut, kUncut, 0, 0, nullptr, nullptr};
-  // two blocks an SM, no more (sequences of a packed row: as many tokens for each as if there were one); back three segments, too, where whole
-  // sequences leave most SMs one block and some two: those are then 2/3 as long (192 blocks, 1000 tokens of 32 states: 215 us without, 191 with)
+  // Two blocks for each SM, no more (sequences of a packed row: as many tokens for each as if there were one), also where it has one at a time:
+  // 4096 tokens in 64 blocks, fp32, take 330 us in four segments and 345 in two.  Back three segments, too, where whole sequences leave some SMs
+  // twice as many blocks as the others: those are then 2/3 as long.  us without and with, 1000 tokens: 150 blocks 216 and 168, 197 blocks 220 and 192
+  // (bf16, 16 states; 32 states the same), 262 and 204, 268 and 241 (fp32, 16 states); 8000 tokens: 1609 and 1233, 1613 and 1299; 1953 and 1470,
+  // 1988 and 1704; 64 states 2200 and 1668 (160 blocks), 2235 and 1834 (196).
   const int64_t unit = kParts * kChunk, blocks = (int64_t)tiles * a.rows, sms = std::max(1, sm_count());
   const int64_t segments = backward && blocks > sms && 3 * blocks <= 4 * sms ? 3 : 2 * sms / blocks;
   if (segments >= 2) {
     const int64_t length = std::max<int64_t>(kLeast, ((a.tokens + segments - 1) / segments + unit - 1) / unit * unit);
-    if (a.tokens > (backward ? kLeastBack - 1 : kLeastForward - 1) * length) c.length = (int)length, c.part = c.length / kParts;
+    const int least = backward && resident == 2 ? kLeastOfTwoBlocks : kLeastSegments;
+    if (a.tokens > (least - 1) * length) c.length = (int)length, c.part = c.length / kParts;
   }
   c.slots = slots_of(a, c.length), c.parts = slots_of(a, c.part);
   c.ends = reinterpret_cast<float4*>(ws), c.steps = ws + c.parts * tiles * 4 * kGroup;

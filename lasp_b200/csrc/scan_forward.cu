@@ -8,6 +8,7 @@
 namespace lasp {
 namespace {
 
+constexpr int kResident = 2;   // blocks of an SM
 constexpr int kStages = 8;   // chunks that are here, or on their way, as they are in global memory: j - 1 to j + 5
 template <typename T, int LPC>
 struct Shared {
@@ -184,10 +185,11 @@ cudaError_t launch(const lasp_scan_args& a, cudaStream_t st) {
   using TILE = Tile<LPC>;
   constexpr auto kernel = k_scan_forward<T, LPC>;
   constexpr size_t smem = sizeof(Shared<T, LPC>);
+  static_assert(blocks_of_sm(smem) == kResident, "");
   const cudaError_t err = ready<kernel>(smem);
   if (err != cudaSuccess) return err;
   const int tiles = tiles_of<TILE>(a.channels, a.groups);
-  const Cuts cuts = cuts_of<TILE>(a, tiles, false, static_cast<float*>(a.ws));
+  const Cuts cuts = cuts_of<TILE>(a, tiles, false, kResident, static_cast<float*>(a.ws));
   const bool wide = (a.channels / a.groups) % TILE::kEach == 0 && reads_by<T>(a.u, TILE::kEach) && reads_by<T>(a.dt, TILE::kEach) &&
                     reads_by<T>(a.z, TILE::kEach) && reads_by<T>(a.y, TILE::kEach) && reads_by<T>(a.B, 4) && reads_by<T>(a.C, 4);
   if (cuts.length != kUncut)
@@ -209,7 +211,7 @@ cudaError_t forward_as(const lasp_scan_args& a, cudaStream_t st) {
 template <int LPC>
 size_t workspace_as(const lasp_scan_args& a) {
   const int tiles = tiles_of<Tile<LPC>>(a.channels, a.groups);
-  return (size_t)floats_of<Tile<LPC>>(cuts_of<Tile<LPC>>(a, tiles, false, nullptr), tiles) * sizeof(float);
+  return (size_t)floats_of<Tile<LPC>>(cuts_of<Tile<LPC>>(a, tiles, false, kResident, nullptr), tiles) * sizeof(float);
 }
 
 }  // namespace
