@@ -379,7 +379,7 @@ LASP_B200_API int lasp_b200_conv_backward(const lasp_conv_args* a, void* stream)
 
 /* h_t = exp(dt_t[c] A[c][n]) h_(t-1) + dt_t[c] u_t[c] B_t[n],  y_t[c] = (sum_n C_t[n] h_t[c][n] + D[c] u_t[c]) silu(z_t[c]), with
  * dt = softplus(dt + dt_bias) where softplus is set, dt + dt_bias elsewhere; states <= 64.  B and C are shared by the channels /
- * groups channels of a group.  A, D and the states h (sequences, channels, states) are fp32.  A of an infinity counts as fp32's
+ * groups channels of a group.  A and the states h (sequences, channels, states) are fp32.  A of an infinity counts as fp32's
  * largest number.  Backward needs `kept`, which the forward pass leaves (lasp_b200_scan_kept_bytes(); NULL: not wanted). */
 typedef struct {
   int32_t rows, tokens, channels, states, groups;

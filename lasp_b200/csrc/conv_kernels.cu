@@ -4,8 +4,11 @@
 //   dp_t = dy_t silu'(p_t),  dx_t = sum_k w_(W-1-k) dp_(t+k),  dw_j = sum_t dp_t x_(t-W+1+j)
 //
 // A thread owns V neighbouring channels and a run of tokens: the last W - 1 inputs slide through its registers, so that every input is
-// read once but for the W - 1 ahead of a run.  Nothing is staged.  Memory and the issue of instructions bound it: forward
-// 8 x 2048 x 4096 bf16 66 us (41 us at the copy rate), backward 131 us (62).
+// read once but for the W - 1 ahead of a run.  Nothing is staged.  The latency of loads bounds it, nothing is near its limit: 8 x 2048 x 4096
+// bf16 takes 62 us forward (41 at the copy rate; DRAM 45 % busy, issue slots and the pipe of exponentials and conversions 53 %, 34 of 64 warps an SM)
+// and 128 backward (62; 38, 53 and 26 %, 29 warps), fp16 62 and 148, fp32 with as many bytes (4 x 2048 x 4096) 55 and 92.  Registers for five and
+// four blocks an SM are paid for with spills, in bytes stored and loaded by a thread: forward 32 and 64 (16 bits), 108 and 260 (fp32); backward
+// 52 and 80 (bf16), 56 and 84 (fp16), 112 and 260 (fp32).
 #include <algorithm>
 #include <type_traits>
 
@@ -483,7 +486,7 @@ cudaError_t backward_of(const lasp_conv_args& a, cudaStream_t st) {
 }
 
 // Channels of a thread.  Eight need 250 registers: 8 x 2048 x 4096 bf16 took 177 us forward and 552 backward, four 76 and 179, a pair (packed
-// arithmetic, five and four blocks an SM) 66 and 131.
+// arithmetic, five and four blocks an SM) 62 and 128.
 constexpr int kPair = 2;
 template <typename T>
 cudaError_t dispatch(const lasp_conv_args& a, bool backward, cudaStream_t st) {

@@ -2,7 +2,7 @@
 //
 // One barrier a chunk: while the first four warps take chunk j through the recurrence, the next four prepare chunk j + 2 (step sizes, inputs,
 // B and C as numbers), and the last four finish chunk j - 1 (gate, output), send for chunk j + 5 and wait for chunk j + 3.  Measured, 16 states,
-// bf16: 2 x 2048 x 4096 140 us (256 blocks on 148 SMs; 20 us of memory, 30 of exponentials), 1 x 16384 x 4096 598 (128 blocks; 82, 238).
+// bf16: 2 x 2048 x 4096 140 us (256 blocks on 148 SMs; 20 us of memory, 60 of exponentials), 1 x 16384 x 4096 598 (128 blocks; 82, 238).
 #include "scan_common.cuh"
 
 namespace lasp {

@@ -1,6 +1,6 @@
 // Selective scan for single tokens: every row of a decoding batch reads the state of its sequence, takes it one token on and writes
-// it back.  Memory bounds it, 8 bytes for every state; B, C and what belongs to a channel are small beside it.  256 rows of 4096 channels and 16 states,
-// bf16: 33 us, 66 % of the copy rate (instructions keep it from more: 55 % of the issue slots); one row of 2048 channels: 7 us, a launch.
+// it back.  Its floor is memory, 8 bytes for every state; B, C and what belongs to a channel are small beside it.  256 rows of 4096 channels and 16 states,
+// bf16: 33 us, 66 % of the copy rate (with 55 % of the issue slots busy: latency, one row's state being under way a block); one row of 2048 channels: 7 us, a launch.
 #include "scan_common.cuh"
 
 namespace lasp {
@@ -12,7 +12,8 @@ constexpr int kOwn = 4;                              // channels of a lane, side
 // A lane holds 4 states of each of its channels; LPC lanes side by side have those of a channel.  The state of the next row is sent for
 // before this one's is worked on.  What belongs to a channel and token (step, input, gate) is worked out by one lane and handed round.
 // WHOLE: every lane has four states of four channels of one group, reads the states, B and C by four, and numbers and pitches have 32
-// bits; checks for less than that and 64-bit products were half of all instructions.
+// bits; checks for less than that and 64-bit products were half of all instructions.  Other numbers of states than 16, 32 and 64 take the
+// variant with the checks, which spills (36 to 64 bytes a thread): 256 rows of 4096 channels take 53 us with 8 states and 59 with 12, 35 with 16.
 template <typename T, int LPC, bool WHOLE>
 __global__ void __launch_bounds__(kStepThreads, kStepBlocks) k_scan_step(lasp_scan_step_args a, int per) {
   __shared__ StepRows rows;

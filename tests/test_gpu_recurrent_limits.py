@@ -76,7 +76,8 @@ def test_a_state_of_zero_stays_so_where_a_part_grows_beyond_fp32():
 def test_long_rows_lose_no_bits(b, n, c):
     """Decays between a half and one, states with a hundred tokens' memory.  Relative errors in the norm: some 100 roundings of 2^-25 on
     average each for decays and for states, in no order, are 10 x 2.4e-8 each, and the sums of a result as much again, 4e-7 together; a decay that
-    is 2e-8 low on average, as the hardware's exponential is, makes 100 x 2e-8 of it, sums with less than 22 bits more than that."""
+    is 2e-8 low on average, as the hardware's exponential is, makes 100 x 2e-8 of it, sums with less than 22 bits more than that.  dA is a sum
+    of products of a state and a gradient that have each come through such a row: twice of either."""
     from lasp_b200 import selective_scan
     g = torch.Generator(device=DEV).manual_seed(n)
     N = 16
@@ -88,7 +89,7 @@ def test_long_rows_lose_no_bits(b, n, c):
     got = {"y": y.detach(), "state": last.detach(), **dict(zip(("du", "ddt", "dA", "dB", "dC", "dinitial"), grads))}
     want = F.scan(**t)
     off = {k: float((got[k].double() - want[k]).norm() / want[k].norm()) for k in got}
-    assert all(v < 1e-6 for v in off.values()), off
+    assert all(v < (2e-6 if k == "dA" else 1e-6) for k, v in off.items()), off
 
 
 # ---- blocks of several rows ----------------------------------------------------------------------------------------------------
